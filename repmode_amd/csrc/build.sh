@@ -5,7 +5,8 @@ HERE="$(cd "$(dirname "${BASH_SOURCE[0]}")" && pwd)"
 ROOT="$(cd "$HERE/../.." && pwd)"
 OUT="${REPMODE_OUT:-$HERE/../librepmode_hip.so}"      # (REPMODE_OUT / REPMODE_BUILD_DIR: a variant build next to the product one)
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -I$ROOT/include -I$HERE ${REPMODE_EXTRA_FLAGS:-}"
+# (packed float32 instructions off: some of their forms have given wrong results on this hardware)
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -I$ROOT/include -I$HERE ${REPMODE_EXTRA_FLAGS:-}"
 BUILD="${REPMODE_BUILD_DIR:-$HERE/build}"
 mkdir -p "$BUILD"
 pids=()
@@ -13,7 +14,7 @@ objs=()
 for f in "$HERE"/*.hip; do
   o="$BUILD/$(basename "${f%.hip}").o"
   objs+=("$o")
-  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ "$HERE/common.h" -nt "$o" ] || [ "$HERE/tail_jobs.h" -nt "$o" ] || [ "$HERE/box_body.h" -nt "$o" ] || [ "$HERE/wgrad_col.h" -nt "$o" ] || [ "$ROOT/include/repmode_hip.h" -nt "$o" ]; then
+  if [ ! -f "$o" ] || [ "$f" -nt "$o" ] || [ "$HERE/build.sh" -nt "$o" ] || [ "$HERE/common.h" -nt "$o" ] || [ "$HERE/tail_jobs.h" -nt "$o" ] || [ "$HERE/box_body.h" -nt "$o" ] || [ "$HERE/wgrad_col.h" -nt "$o" ] || [ "$ROOT/include/repmode_hip.h" -nt "$o" ]; then
     $HIPCC $FLAGS -c "$f" -o "$o" &
     pids+=($!)
   fi
