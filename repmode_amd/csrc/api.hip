@@ -38,6 +38,30 @@ int repmode_reserve_cus() { return g_reserve_cus; }
 extern "C" int repmode_set_reserve_cus(int n) { g_reserve_cus = n > 0 ? n : 0; return REPMODE_OK; }
 extern "C" int repmode_get_reserve_cus(void) { return g_reserve_cus; }
 
+// Zeros by a kernel of our own: a hipMemsetAsync that a caller captures becomes a memset node, and graphs with such nodes have been
+// seen to leave the memory as it was on replays after the first.  Float buffers: a multiple of 4 bytes at a multiple of 4.
+namespace {
+__global__ __launch_bounds__(256) void clear_kernel(uint32_t* __restrict__ p, size_t head, size_t n16, size_t words) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n16) reinterpret_cast<u32x4*>(p + head)[i] = u32x4{0, 0, 0, 0};
+  if (i < head) p[i] = 0;
+  const size_t tail = head + 4 * n16 + i;
+  if (i < 4 && tail < words) p[tail] = 0;
+}
+}  // namespace
+int repmode_clear(void* p, size_t bytes, hipStream_t s) {
+  RM_REQUIRE((((uintptr_t)p | bytes) & 3) == 0, "clear: a float buffer");
+  const size_t words = bytes / 4;
+  if (words == 0) return REPMODE_OK;
+  size_t head = ((16 - ((uintptr_t)p & 15)) & 15) / 4;
+  if (head > words) head = words;
+  const size_t n16 = (words - head) / 4, blocks = (n16 + 255) / 256;
+  RM_REQUIRE(blocks < (1UL << 31), "clear: buffer too large");
+  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks ? blocks : 1)), dim3(256), 0, s, static_cast<uint32_t*>(p), head, n16, words);
+  RM_LAUNCH_CHECK("clear");
+  return REPMODE_OK;
+}
+
 extern "C" int repmode_abi_version(void) { return REPMODE_ABI_VERSION; }
 extern "C" const char* repmode_last_error(void) { return g_err; }
 
@@ -112,8 +136,8 @@ float* repmode_zero_scratch(hipStream_t s) {
   float* p = nullptr;
   const size_t bytes = (REPMODE_ZERO_SCRATCH_FLOATS + REPMODE_SCRATCH_TAIL_WORDS) * sizeof(float);
   hipError_t e = hipMalloc(&p, bytes);
-  if (e == hipSuccess) e = hipMemsetAsync(p, 0, bytes, s);
   if (e != hipSuccess) { repmode_set_error("zero_scratch: %s", hipGetErrorString(e)); return nullptr; }
+  if (repmode_clear(p, bytes, s) != REPMODE_OK) return nullptr;
   g_scratch[{dev, s}] = p;
   return p;
 }

@@ -42,6 +42,13 @@ void repmode_set_error(const char* fmt, ...);
     }                                                                        \
   } while (0)
 
+// zeros on the stream by a kernel (api.hip), also inside a captured graph; bytes: a multiple of 4
+int repmode_clear(void* p, size_t bytes, hipStream_t s);
+#define RM_CLEAR(args)                          \
+  do {                                          \
+    if (int rc__ = repmode_clear args) return rc__; \
+  } while (0)
+
 __device__ __forceinline__ float bf16_to_f32(bf16_t v) { return __uint_as_float(((uint32_t)v) << 16); }
 
 // round-to-nearest-even, NaN kept quiet

@@ -307,7 +307,7 @@ int launch_deep(DeepArgs a, bool y_is_zero, hipStream_t stream) {
     attr_set.fetch_or(1u << (dev & 31), std::memory_order_release);
   }
   if (!y_is_zero)
-    RM_HIP(hipMemsetAsync(a.y, 0, (size_t)(TWO_IN ? 1 : 2) * a.N * a.D * a.H * a.W * a.Cout * sizeof(float), stream));
+    RM_CLEAR((a.y, (size_t)(TWO_IN ? 1 : 2) * a.N * a.D * a.H * a.W * a.Cout * sizeof(float), stream));
   // algorithmic FLOPs = the layer's merged 125-tap convolution, once per layer and direction; the 3x3x3
   // expert's 27 taps are executed work, not algorithmic
   const double alg = 2.0 * a.N * a.D * a.H * a.W * (double)a.Cin * a.Cout * REPMODE_TAPS;

@@ -1847,8 +1847,8 @@ int launch_cfg(ConvArgs a, hipStream_t stream) {
   }
   if ((ks > 1 || a.ksplit > 1 || (a.dual && !(a.dual & 4))) && !a.accum) {
     const size_t vox = (size_t)((a.dual & 4) ? 2 * a.N : a.N) * a.D * a.H * a.W;
-    RM_HIP(hipMemsetAsync(a.y, 0, vox * (a.Cout1 > 0 ? a.Cout1 : a.Cout) * sizeof(float), stream));
-    if (a.Cout1 > 0) RM_HIP(hipMemsetAsync(a.y2, 0, vox * (a.Cout - a.Cout1) * sizeof(float), stream));
+    RM_CLEAR((a.y, vox * (a.Cout1 > 0 ? a.Cout1 : a.Cout) * sizeof(float), stream));
+    if (a.Cout1 > 0) RM_CLEAR((a.y2, vox * (a.Cout - a.Cout1) * sizeof(float), stream));
   }
   // algorithmic FLOPs = the layer's merged 125-tap convolution, counted ONCE per layer and direction: a
   // launch restricted to the 3x3x3 support is the per-expert formulation's second conv of a layer whose 125 taps

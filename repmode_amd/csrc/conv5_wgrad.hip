@@ -1211,7 +1211,7 @@ int launch_wgrad_bf16(WgradArgs a, int n, hipStream_t s) {
       if (a.plan_out) { *a.plan_out = 0; return REPMODE_OK; }     // (shared units are added with float atomics)
       a.sk_total = total;
       a.nchunks = 1; a.tiles_per_block = a.ntiles; a.direct = 0;
-      if (!a.prezeroed) RM_HIP(hipMemsetAsync(a.dw, 0, (size_t)a.nslots * REPMODE_TAPS * a.Cout * a.CinTot * sizeof(float), s));
+      if (!a.prezeroed) RM_CLEAR((a.dw, (size_t)a.nslots * REPMODE_TAPS * a.Cout * a.CinTot * sizeof(float), s));
       repmode_prof_begin(REPMODE_PROF_WGRAD, 2.0 * n * a.D * a.H * a.W * (double)a.Cin * a.Cout * REPMODE_TAPS, s);
       if constexpr (TX >= 16 && TZ == 1)
         hipLaunchKernelGGL((conv5_wgrad_bf16_kernel<TZ, TY, TX, true, false, true>), dim3((unsigned)g), dim3(512), 0, s, a);
@@ -1258,12 +1258,12 @@ int launch_wgrad_bf16(WgradArgs a, int n, hipStream_t s) {
   };
   long grid = plan(a.ndz, a.layout, &a.tiles_per_block, &a.nchunks, &a.direct);
   if (a.plan_out) { *a.plan_out = a.direct && !a.dy2; return REPMODE_OK; }
-  if (!a.direct && !a.prezeroed) RM_HIP(hipMemsetAsync(a.dw, 0, (size_t)a.nslots * (a.layout == 2 ? 27 : REPMODE_TAPS) * a.Cout * a.CinTot * sizeof(float), s));
+  if (!a.direct && !a.prezeroed) RM_CLEAR((a.dw, (size_t)a.nslots * (a.layout == 2 ? 27 : REPMODE_TAPS) * a.Cout * a.CinTot * sizeof(float), s));
   if (a.dy2) {                       // dual launch: the second job is planned the same way, its workgroups follow the first's
     a.grid0 = (int)grid;
     grid += plan(a.ndz2, a.layout2, &a.tiles_per_block2, &a.nchunks2, &a.direct2);
     RM_REQUIRE(a.layout2 == 0 || a.direct2, "conv5_wgrad_dual: job 2 cannot write the expert layout with atomics");
-    if (!a.direct2 && !a.prezeroed) RM_HIP(hipMemsetAsync(a.dw2, 0, (size_t)REPMODE_TAPS * a.Cout * a.CinTot * sizeof(float), s));
+    if (!a.direct2 && !a.prezeroed) RM_CLEAR((a.dw2, (size_t)REPMODE_TAPS * a.Cout * a.CinTot * sizeof(float), s));
   }
   RM_REQUIRE(grid < (1L << 31), "conv5_wgrad: grid too large");
   repmode_prof_begin(REPMODE_PROF_WGRAD, 2.0 * n * a.D * a.H * a.W * (double)a.Cin * a.Cout * REPMODE_TAPS, s);
@@ -1388,7 +1388,7 @@ extern "C" int repmode_conv5_wgrad_part(const void* x, const void* dy, const int
     a.direct = a.nchunks == 1;
     const long grid = fixed * a.nchunks;
     RM_REQUIRE(grid < (1L << 31), "conv5_wgrad: grid too large");
-    if (!a.direct && !a.prezeroed) RM_HIP(hipMemsetAsync(dw, 0, (size_t)nslots * (a.layout == 2 ? 27 : REPMODE_TAPS) * cout * a.CinTot * sizeof(float), s));
+    if (!a.direct && !a.prezeroed) RM_CLEAR((dw, (size_t)nslots * (a.layout == 2 ? 27 : REPMODE_TAPS) * cout * a.CinTot * sizeof(float), s));
     repmode_prof_begin(REPMODE_PROF_WGRAD, 2.0 * n * d * h * wdim * (double)cin * cout * REPMODE_TAPS, s);
     hipLaunchKernelGGL(conv5_wgrad_f32c_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, a);
   }
@@ -1720,7 +1720,7 @@ extern "C" int repmode_conv5_wgrad_thin(const void* a_t, const void* b_t, const 
   if (repmode_deterministic() && want > repmode_det_cap(RM_DET_WGRAD)) want = repmode_det_cap(RM_DET_WGRAD);      // (deterministic: at most two addends per element of the cleared dw)
   a.tiles_per_block = ceil_div(a.ntiles, (int)want);
   a.nchunks = ceil_div(a.ntiles, a.tiles_per_block);
-  if (!(flip & 2)) RM_HIP(hipMemsetAsync(dw, 0, (size_t)nslots * REPMODE_TAPS * c * sizeof(float), s));   // flip bit 1: dw already cleared
+  if (!(flip & 2)) RM_CLEAR((dw, (size_t)nslots * REPMODE_TAPS * c * sizeof(float), s));   // flip bit 1: dw already cleared
   repmode_prof_begin(REPMODE_PROF_WGRAD_THIN, 2.0 * n * d * h * wdim * (double)c * REPMODE_TAPS, s);
   hipLaunchKernelGGL(conv5_wgrad_thin_kernel, dim3((unsigned)(fixed * a.nchunks)), dim3(256), 0, s, a);
   repmode_prof_end(s);

@@ -604,7 +604,7 @@ int launch_col(const WgColCall& c, hipStream_t s) {
   }
   if (c.plan_out) { *c.plan_out = direct ? 1 : 0; return REPMODE_OK; }
   if (!direct && !c.prezeroed)
-    RM_HIP(hipMemsetAsync(c.dw, 0, (size_t)c.nslots * REPMODE_TAPS * c.Cout * c.CinTot * sizeof(float), s));
+    RM_CLEAR((c.dw, (size_t)c.nslots * REPMODE_TAPS * c.Cout * c.CinTot * sizeof(float), s));
   repmode_prof_begin(REPMODE_PROF_WGRAD, 2.0 * c.N * c.D * c.H * c.W * (double)c.Cin * c.Cout * REPMODE_TAPS, s);
   hipLaunchKernelGGL((conv5_wgrad_col_kernel<TY, TX, SPS, RING, DUAL, Q>), dim3((unsigned)g), dim3(512), 0, s, a);
   return REPMODE_OK;

@@ -259,7 +259,7 @@ extern "C" int repmode_expert_mix_bwd_ex(const float* dy, const float* p, const 
   RM_REQUIRE(dy && p && g && dg && dye_lo && dye_hi && n > 0 && v > 0 && c > 0 && c <= 512, "expert_mix_bwd: bad argument");
   RM_REQUIRE(dtype == REPMODE_F32 || dtype == REPMODE_BF16, "expert_mix_bwd: bad dtype %d", dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!prezeroed) RM_HIP(hipMemsetAsync(dg, 0, (size_t)n * E * c * sizeof(float), s));
+  if (!prezeroed) RM_CLEAR((dg, (size_t)n * E * c * sizeof(float), s));
   const int rows = 256 / ((c + 3) / 4);
   // RM_MIX_ITERS row iterations per workgroup (level 3, in the step: 4 iterations on 128 workgroups 17.5 us; 1 iteration on
   // 512 workgroups 22.1 us -- every workgroup ends in 5 C float atomics on the sample's gate gradients)
@@ -301,7 +301,7 @@ extern "C" int repmode_expert_mix_bwd_box(const float* dy, const float* p, const
       if (v * t * 4 * 4 <= 64 * 1024 && v * (t / 4) <= 256 * BOX_MAXI && d < 1024 && h < 1024 && w < 1024) { cb = t; break; }
   RM_REQUIRE(cb > 0, "expert_mix_bwd_box: the volume does not fit in LDS (or c %% 4 != 0)");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!prezeroed) RM_HIP(hipMemsetAsync(dg, 0, (size_t)n * E * c * sizeof(float), s));
+  if (!prezeroed) RM_CLEAR((dg, (size_t)n * E * c * sizeof(float), s));
   const int rows = 256 / ((c + 3) / 4);
   long chunks = (v + rows * RM_MIX_ITERS - 1) / (rows * RM_MIX_ITERS);
   if (chunks > 256) chunks = 256;

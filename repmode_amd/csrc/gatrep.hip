@@ -1135,7 +1135,7 @@ extern "C" int repmode_gatrep_bwd_ex(const float* dw, const float* k5, const flo
     dg += REPMODE_SCRATCH_GATE_OFF;
     clear = 1;
   } else {
-    RM_HIP(hipMemsetAsync(dg_ws, 0, ndg * sizeof(float), s));
+    RM_CLEAR((dg_ws, ndg * sizeof(float), s));
   }
   repmode_prof_begin(REPMODE_PROF_GATREP_BWD, (double)co * ci * 4.0 * (125.0 * nslots + 2 * 155.0), s);
   // Small layers (at most one workgroup per CU) are one dependent chain per launch: 512 threads per tile, 8 slots' loads in

@@ -580,7 +580,7 @@ extern "C" int repmode_k2s2_wgrad_ex(const void* coarse, const void* fine, float
     if (repmode_deterministic() && chunks > repmode_det_cap(RM_DET_K2S2)) chunks = repmode_det_cap(RM_DET_K2S2);      // (deterministic: at most two addends per element of the cleared dw)
     f.rows_per_block = (int)(((f.M + chunks - 1) / chunks + 31) / 32 * 32);
     const int nchunks_f = (int)((f.M + f.rows_per_block - 1) / f.rows_per_block);
-    if (!prezeroed && nchunks_f > 1) RM_HIP(hipMemsetAsync(dw, 0, (size_t)8 * ca * cb * sizeof(float), s));
+    if (!prezeroed && nchunks_f > 1) RM_CLEAR((dw, (size_t)8 * ca * cb * sizeof(float), s));
     hipLaunchKernelGGL(k2s2_wgrad_f32_kernel, dim3(nchunks_f, tiles, 8), dim3(256), 0, s, f);
     RM_LAUNCH_CHECK("k2s2_wgrad_f32");
     return REPMODE_OK;
@@ -621,7 +621,7 @@ extern "C" int repmode_k2s2_wgrad_ex(const void* coarse, const void* fine, float
   a.tiles_per_block = ceil_div(a.ntiles, (int)want);
   const int nchunks = ceil_div(a.ntiles, a.tiles_per_block);
   a.direct = nchunks == 1;
-  if (!prezeroed && !a.direct) RM_HIP(hipMemsetAsync(dw, 0, (size_t)8 * ca * cb * sizeof(float), s));
+  if (!prezeroed && !a.direct) RM_CLEAR((dw, (size_t)8 * ca * cb * sizeof(float), s));
   const bool vec = (ca & 7) == 0 && (cb & 7) == 0 && a.M * (long)ca * 2 < (1L << 31) && a.M * 8 * (long)cb * 2 < (1L << 31);
   if (vec) hipLaunchKernelGGL(k2s2_wgrad_kernel<true>, dim3(nchunks, nat, nbt), dim3(KW_NT), 0, s, a);
   else hipLaunchKernelGGL(k2s2_wgrad_kernel<false>, dim3(nchunks, nat, nbt), dim3(KW_NT), 0, s, a);
