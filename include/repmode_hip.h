@@ -497,6 +497,58 @@ int repmode_adam_expert_frags_dev(int nblocks, float* const* p5, const float* co
                                   float* const* p3, const float* const* g3, float* const* m3, float* const* v3, const int* co,
                                   const int* ci, void* const* wf, void* const* wd, const float* hyper_dev, void* stream);
 
+/* ---- AdamW (decoupled weight decay) over a list of tensors, moments in float32 or in 8 bits (csrc/adamw.hip) ----
+ * Per element, float32, g' = clip * g (fnet_model.py:55, 112 step plain Adam: weight_decay 0, no clip):
+ *   m += (1 - beta1)(g' - m);  v = beta2 v + (1 - beta2) g'^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * Pointer arguments are HOST arrays of ntensors device pointers; tensors are flat and dense and do not overlap.
+ *   dtype       of parameters and gradients: float32, or bfloat16 (the update is float32 and rounded once, stochastically)
+ *   state_bits  32: m, v float32, the scales are not read (NULL).  8: m holds e4m3 and v e5m2 codes, one byte an element;
+ *               m_scale / v_scale one e8m0 byte (2^(byte - 127), 1 .. 254) for every REPMODE_ADAMW_BLOCK elements or part of them.
+ *               Zero moments: zero codes with any scale.
+ *   position    of each tensor in the caller's whole list: with seed and step it decides the stochastic roundings' random bits
+ *   step        the 1-based count of this update.  hyper_dev != NULL: a captured step -- lr .. seed are not read, the
+ *               constants come from device memory (REPMODE_ADAMW_HYPER_FLOATS floats, 16-byte aligned) as
+ *               repmode_adamw_hyper_dev leaves them: it advances *step_dev (int64) and takes lr from lr_dev where that is given.
+ *   clip        device scalar or NULL (1).  NaN: parameters and moments stay as they are. */
+#define REPMODE_ADAMW_MAX 60
+#define REPMODE_ADAMW_BLOCK 256
+#define REPMODE_ADAMW_HYPER_FLOATS 8
+int repmode_adamw_multi(int ntensors, int dtype, int state_bits, void* const* p, const void* const* g, void* const* m,
+                        void* const* m_scale, void* const* v, void* const* v_scale, const long* numel, const int* position, double lr,
+                        double beta1, double beta2, double eps, double weight_decay, long step, unsigned long seed,
+                        const float* hyper_dev, const float* clip, void* stream);
+int repmode_adamw_hyper_dev(long* step_dev, float* hyper_dev, double lr, const float* lr_dev, double beta1, double beta2, double eps,
+                            double weight_decay, unsigned long seed, void* stream);
+
+/* ---- the norm of many tensors together (csrc/grad_norm.hip) ----
+ * partial: writes one float64 sum of squares per REPMODE_GRAD_NORM_CHUNK bytes (or part of them) of every tensor into
+ *   partial[0 .. *used); capacity: the room there.  Lists longer than REPMODE_GRAD_NORM_MAX, or of two dtypes, take several
+ *   calls that write one behind the other.
+ * finish: norm = sqrt(sum of n partials), clip = min(1, max_norm / (norm + 1e-6)) or NaN where the sum is not finite. */
+#define REPMODE_GRAD_NORM_MAX 200
+#define REPMODE_GRAD_NORM_CHUNK 32768
+int repmode_grad_norm_partial(int ntensors, int dtype, const void* const* x, const long* numel, double* partial, long capacity,
+                              long* used, void* stream);
+int repmode_grad_norm_finish(const double* partial, long n, double max_norm, float* norm, float* clip, void* stream);
+
+/* ---- load-balance loss of a router or of a mixture's gates, per-expert counts, gradient (csrc/balance.hip) ----
+ * x: logits [groups][rows][experts] with element strides sg, sn, se, float32 or bfloat16; mask: bytes [groups][rows] with strides
+ * mg, mn, 0 = the row does not count (it is not read), or NULL.  A row of -inf alone does not count either.  With p = softmax(x),
+ * the top_k largest of each row chosen (ties: the lowest index; never a -inf), f_ge the share of group g's choices that are e and
+ * P_ge the mean of its p_e:  loss = coef * experts * mean over the groups that have rows of sum_e f_ge P_ge.
+ *   counts int64, prob float [groups][experts]: choices, mean probabilities.  weight: float [groups * experts + 1], for the
+ *   backward pass.  ws: repmode_balance_plan's bytes, 8-byte aligned.
+ * bwd: dx = *up * d loss / d x (up: device scalar; counts are constants), rows that do not count get 0; strides dg, dn, de. */
+#define REPMODE_BALANCE_MAX_EXPERTS 1024
+int repmode_balance_plan(long groups, long rows, int experts, long* ws_bytes);
+int repmode_balance_fwd(const void* x, int dtype, long groups, long rows, int experts, long sg, long sn, long se,
+                        const unsigned char* mask, long mg, long mn, int top_k, double coef, void* ws, long ws_bytes, float* loss,
+                        long* counts, float* prob, float* weight, void* stream);
+int repmode_balance_bwd(const void* x, int dtype, long groups, long rows, int experts, long sg, long sn, long se,
+                        const unsigned char* mask, long mg, long mn, const float* weight, const float* up, void* dx, long dg, long dn,
+                        long de, void* stream);
+
 /* Developer / test switch of the convolution's pipelined form (csrc/conv5_igemm.hip, conv5_pipe_kernel; also REPMODE_CONV_PIPE):
  * bit 0 = on, bit 1 = one channel sub-tile per wave everywhere, bit 2 = also on grids smaller than the chip, bit 3 = the
  * wave-specialised kernel (MFMA waves + loader waves),  bit 4 = its items along z first, bit 5 = row-stationary tap

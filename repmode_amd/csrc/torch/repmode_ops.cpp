@@ -18,7 +18,9 @@
 #include <torch/autograd.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdlib>
 #include <memory>
 #include <mutex>
@@ -1815,6 +1817,222 @@ void op_adam_step_dev(const std::vector<Tensor>& params, const std::vector<Tenso
   adam_step_impl(params, grads, exp_avgs, exp_avg_sqs, lr, beta1, beta2, eps, 0, &step_dev, &hyper_dev);
 }
 
+// ------------------------------------------------------------------------------------------------------------
+// The norm of many tensors and AdamW over many tensors (csrc/grad_norm.hip, csrc/adamw.hip).
+// A tensor is flat here: its elements in memory order, so it has to be dense, and a gradient of other strides than its
+// parameter's is brought into the parameter's order first.
+std::tuple<Tensor, Tensor> op_grad_norm(const std::vector<Tensor>& tensors, double max_norm) {
+  TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
+  TORCH_CHECK(max_norm >= 0, "grad_norm: max_norm must not be negative or NaN, got ", max_norm);
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const Tensor& t = tensors[i];
+    require_hip(t, "grad_norm: tensor");
+    (void)dtype_code(t.scalar_type());
+    TORCH_CHECK(t.device() == tensors[0].device(), "grad_norm: tensor ", i, " is on ", t.device(), ", tensor 0 on ", tensors[0].device());
+  }
+  DeviceGuard guard(tensors[0].device());
+  at::NoGradGuard no_grad;
+  std::vector<const void*> x[2];
+  std::vector<long> numel[2];
+  std::vector<Tensor> hold;
+  long room = 0;
+  for (const Tensor& t0 : tensors) {
+    if (t0.numel() == 0) continue;
+    Tensor t = t0;
+    if (!t.is_non_overlapping_and_dense()) hold.push_back(t = t0.contiguous());        // (any order of the elements has the same norm)
+    const int code = dtype_code(t.scalar_type());
+    x[code].push_back(t.data_ptr());
+    numel[code].push_back((long)t.numel());
+    const long per = REPMODE_GRAD_NORM_CHUNK / t.element_size();
+    room += (t.numel() + per - 1) / per;
+  }
+  auto f32 = tensors[0].options().dtype(at::kFloat);
+  Tensor out = at::empty({2}, f32), partial = at::empty({std::max(room, 1L)}, f32.dtype(at::kDouble));
+  double* at_ = partial.data_ptr<double>();
+  long used = 0;
+  for (int code : {REPMODE_F32, REPMODE_BF16})
+    for (size_t b = 0; b < x[code].size(); b += REPMODE_GRAD_NORM_MAX) {
+      const int cnt = (int)std::min<size_t>(REPMODE_GRAD_NORM_MAX, x[code].size() - b);
+      long n = 0;
+      RM_CALL(repmode_grad_norm_partial, cnt, code, x[code].data() + b, numel[code].data() + b, at_ + used, room - used, &n, stream_handle());
+      used += n;
+    }
+  RM_CALL(repmode_grad_norm_finish, at_, used, max_norm, out.data_ptr<float>(), out.data_ptr<float>() + 1, stream_handle());
+  return {out.select(0, 0), out.select(0, 1)};
+}
+
+// A parameter's moments are float32 (its scales are not looked at), or 8-bit with one power of two per REPMODE_ADAMW_BLOCK elements
+// in exp_avg_scales / exp_avg_sq_scales; both lists may be empty where no moments are 8-bit.  step_dev: a step that is captured.
+void op_adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs,
+                   const std::vector<Tensor>& exp_avg_scales, const std::vector<Tensor>& exp_avg_sqs,
+                   const std::vector<Tensor>& exp_avg_sq_scales, double lr, double beta1, double beta2, double eps, double weight_decay,
+                   int64_t step, const OptTensor& step_dev, const OptTensor& lr_dev, const OptTensor& clip, int64_t seed) {
+  const size_t n = params.size();
+  TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && exp_avg_scales.size() == exp_avg_sq_scales.size() &&
+                  (exp_avg_scales.empty() || exp_avg_scales.size() == n), "adamw_step: list lengths differ");
+  if (n == 0) return;
+  const at::Device dev = params[0].device();
+  std::vector<std::pair<const char*, const char*>> spans;      // what is written
+  spans.reserve(n * (exp_avg_scales.empty() ? 3 : 5));
+  auto span = [&](const Tensor& t) {
+    if (t.numel()) spans.emplace_back(static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes());
+  };
+  auto same_order = [](const Tensor& t, const Tensor& p) { return t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous()); };
+  std::vector<char> eight(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    const at::ScalarType dt = p.scalar_type();
+    require_hip(p, "adamw_step: a parameter");
+    (void)dtype_code(dt);
+    TORCH_CHECK(p.device() == dev && p.is_non_overlapping_and_dense(), "adamw_step: parameter ", i, ": dense tensors on one device");
+    TORCH_CHECK(grads[i].layout() == at::kStrided && grads[i].device() == dev && grads[i].scalar_type() == dt && grads[i].sizes() == p.sizes(),
+                "adamw_step: gradient ", i, ": the parameter's type, shape and device");
+    eight[i] = exp_avgs[i].scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK(exp_avgs[i].scalar_type() == (eight[i] ? at::kFloat8_e4m3fn : at::kFloat) &&
+                    exp_avg_sqs[i].scalar_type() == (eight[i] ? at::kFloat8_e5m2 : at::kFloat),
+                "adamw_step: moments of parameter ", i, ": both float32, or float8_e4m3fn and float8_e5m2");
+    for (const Tensor* s : {&exp_avgs[i], &exp_avg_sqs[i]}) {
+      TORCH_CHECK(s->device() == dev && s->sizes() == p.sizes() && same_order(*s, p),
+                  "adamw_step: moments of parameter ", i, ": its shape, strides and device");
+      span(*s);
+    }
+    span(p);
+    if (!eight[i]) continue;
+    TORCH_CHECK(!exp_avg_scales.empty(), "adamw_step: 8-bit moments need their scales");
+    for (const Tensor* s : {&exp_avg_scales[i], &exp_avg_sq_scales[i]}) {
+      TORCH_CHECK(s->device() == dev && s->scalar_type() == at::kFloat8_e8m0fnu && s->is_contiguous() &&
+                      s->numel() == (p.numel() + REPMODE_ADAMW_BLOCK - 1) / REPMODE_ADAMW_BLOCK,
+                  "adamw_step: scales of parameter ", i, ": one contiguous float8_e8m0fnu value per ", REPMODE_ADAMW_BLOCK, " elements");
+      span(*s);
+    }
+  }
+  // what is written is written once: a tensor given twice, or two views of the same memory, would race
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i].first >= spans[i - 1].second, "adamw_step: two of the parameters and moments share memory");
+  auto one = [&](const OptTensor& t, at::ScalarType want, const char* what) {
+    if (!t.has_value() || !t->defined()) return;
+    TORCH_CHECK(t->device() == dev && t->scalar_type() == want && t->numel() == 1, "adamw_step: ", what, ": one ", want, " value on the parameters' device");
+  };
+  one(clip, at::kFloat, "clip");
+  one(lr_dev, at::kFloat, "a learning rate on the device");
+  one(step_dev, at::kLong, "a step count on the device");
+  const bool captured = step_dev.has_value() && step_dev->defined(), lr_on_dev = lr_dev.has_value() && lr_dev->defined();
+  TORCH_CHECK(captured || !lr_on_dev, "adamw_step: a learning rate on the device needs the step count on the device too");
+  const float* clip_p = clip.has_value() && clip->defined() ? clip->data_ptr<float>() : nullptr;
+  DeviceGuard guard(dev);
+  at::NoGradGuard no_grad;
+  Tensor hyper;
+  const float* hd = nullptr;
+  if (captured) {
+    hyper = at::empty({REPMODE_ADAMW_HYPER_FLOATS}, params[0].options().dtype(at::kFloat));
+    RM_CALL(repmode_adamw_hyper_dev, reinterpret_cast<long*>(step_dev->data_ptr<int64_t>()), hyper.data_ptr<float>(), lr,
+            lr_on_dev ? lr_dev->data_ptr<float>() : nullptr, beta1, beta2, eps, weight_decay, (unsigned long)seed, stream_handle());
+    hd = hyper.data_ptr<float>();
+  }
+  // (also where a launch fails half way: some parameters have changed)
+  struct Bump {
+    const std::vector<Tensor>& ps;
+    ~Bump() {
+      for (const Tensor& t : ps)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+  } bump{params};
+  std::vector<Tensor> hold;                                    // gradients brought into their parameters' order
+  for (int kind = 0; kind < 4; ++kind) {                       // (type of the parameter, bits of the moments): a kernel each
+    const int code = kind & 1 ? REPMODE_BF16 : REPMODE_F32;
+    void *p[REPMODE_ADAMW_MAX], *m[REPMODE_ADAMW_MAX], *v[REPMODE_ADAMW_MAX], *ms[REPMODE_ADAMW_MAX], *vs[REPMODE_ADAMW_MAX];
+    const void* g[REPMODE_ADAMW_MAX];
+    long numel[REPMODE_ADAMW_MAX];
+    int position[REPMODE_ADAMW_MAX], cnt = 0;
+    auto flush = [&]() {
+      if (cnt)
+        RM_CALL(repmode_adamw_multi, cnt, code, kind & 2 ? 8 : 32, p, g, m, ms, v, vs, numel, position, lr, beta1, beta2, eps, weight_decay,
+                (long)step, (unsigned long)seed, hd, clip_p, stream_handle());
+      cnt = 0;
+    };
+    for (size_t i = 0; i < n; ++i) {
+      if (params[i].numel() == 0 || (bool)eight[i] != (bool)(kind & 2) || dtype_code(params[i].scalar_type()) != code) continue;
+      const void* gp = grads[i].data_ptr();
+      if (!same_order(grads[i], params[i])) {
+        hold.push_back(at::empty_strided(params[i].sizes(), params[i].strides(), grads[i].options()).copy_(grads[i]));
+        gp = hold.back().data_ptr();
+      }
+      p[cnt] = params[i].data_ptr(); g[cnt] = gp; m[cnt] = exp_avgs[i].data_ptr(); v[cnt] = exp_avg_sqs[i].data_ptr();
+      ms[cnt] = eight[i] ? exp_avg_scales[i].data_ptr() : nullptr;
+      vs[cnt] = eight[i] ? exp_avg_sq_scales[i].data_ptr() : nullptr;
+      numel[cnt] = (long)params[i].numel(); position[cnt] = (int)i;
+      if (++cnt == REPMODE_ADAMW_MAX) flush();
+    }
+    flush();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// The load-balance loss (csrc/balance.hip): logits [groups, rows, experts] or [rows, experts], any strides.
+struct BalanceLoss : public torch::autograd::Function<BalanceLoss> {
+  static variable_list forward(AutogradContext* ctx, Tensor x, OptTensor mask, int64_t top_k, double coef) {
+    DeviceGuard guard(x.device());
+    const bool grouped = x.dim() == 3;
+    const int64_t groups = grouped ? x.size(0) : 1, rows = x.size(-2), experts = x.size(-1);
+    auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
+    auto shape = [&](at::ScalarType t) { return grouped ? at::empty({groups, experts}, f32.dtype(t)) : at::empty({experts}, f32.dtype(t)); };
+    Tensor loss = at::empty({}, f32), prob = shape(at::kFloat), counts = shape(at::kLong), weight = at::empty({groups * experts + 1}, f32);
+    long ws_bytes = 0;
+    RM_CALL(repmode_balance_plan, groups, rows, (int)experts, &ws_bytes);
+    Tensor ws = at::empty({(ws_bytes + 7) / 8}, f32.dtype(at::kDouble));
+    const bool masked = mask.has_value() && mask->defined();
+    RM_CALL(repmode_balance_fwd, x.numel() ? x.data_ptr() : nullptr, dtype_code(x.scalar_type()), groups, rows, (int)experts,
+            grouped ? x.stride(0) : 0, x.stride(-2), x.stride(-1), masked && mask->numel() ? reinterpret_cast<const unsigned char*>(mask->data_ptr<bool>()) : nullptr,
+            masked && grouped ? mask->stride(0) : 0, masked ? mask->stride(-1) : 0, (int)top_k, coef, ws.data_ptr(), ws_bytes, loss.data_ptr<float>(),
+            reinterpret_cast<long*>(counts.data_ptr<int64_t>()), prob.data_ptr<float>(), weight.data_ptr<float>(), stream_handle());
+    ctx->save_for_backward({x, masked ? *mask : Tensor(), weight});
+    ctx->mark_non_differentiable({counts, prob});
+    return {loss, counts, prob};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &x = sv[0], &mask = sv[1], &weight = sv[2];
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    DeviceGuard guard(x.device());
+    const bool grouped = x.dim() == 3, masked = mask.defined();
+    const int64_t groups = grouped ? x.size(0) : 1, rows = x.size(-2), experts = x.size(-1);
+    Tensor up = grads[0].to(at::kFloat), dx = at::empty_like(x);
+    if (x.numel() == 0) return {dx, Tensor(), Tensor(), Tensor()};
+    RM_CALL(repmode_balance_bwd, x.data_ptr(), dtype_code(x.scalar_type()), groups, rows, (int)experts, grouped ? x.stride(0) : 0, x.stride(-2),
+            x.stride(-1), masked ? reinterpret_cast<const unsigned char*>(mask.data_ptr<bool>()) : nullptr, masked && grouped ? mask.stride(0) : 0,
+            masked ? mask.stride(-1) : 0, weight.data_ptr<float>(), up.data_ptr<float>(), dx.data_ptr(), grouped ? dx.stride(0) : 0, dx.stride(-2),
+            dx.stride(-1), stream_handle());
+    return {dx, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// Whether an autograd graph that accumulates into one of these leaves is alive.  Its accumulation nodes belong to the stream of
+// their first use; a backward pass that is captured on another stream would be joined with that stream, which ends the process.
+bool op_graph_alive(const std::vector<Tensor>& leaves) {
+  for (const Tensor& t : leaves)
+    if (t.requires_grad() && t.is_leaf() && torch::autograd::impl::try_get_grad_accumulator(t)) return true;
+  return false;
+}
+
+std::tuple<Tensor, Tensor, Tensor> op_balance_loss(const Tensor& logits, const OptTensor& mask, int64_t top_k, double coef) {
+  require_hip(logits, "balance_loss: logits");
+  (void)dtype_code(logits.scalar_type());
+  TORCH_CHECK(logits.dim() == 2 || logits.dim() == 3, "balance_loss: logits are [rows, experts] or [groups, rows, experts], got ", logits.sizes());
+  const int64_t groups = logits.dim() == 3 ? logits.size(0) : 1, rows = logits.size(-2), experts = logits.size(-1);
+  TORCH_CHECK(groups >= 1 && groups <= 65535 && experts >= 1 && experts <= REPMODE_BALANCE_MAX_EXPERTS,
+              "balance_loss: 1..65535 groups and 1..", REPMODE_BALANCE_MAX_EXPERTS, " experts, got ", logits.sizes());
+  TORCH_CHECK(top_k >= 1 && top_k <= experts, "balance_loss: top_k must be 1..", experts, ", got ", top_k);
+  TORCH_CHECK(rows * top_k < (int64_t(1) << 31), "balance_loss: too many rows in a group: ", rows);
+  TORCH_CHECK(std::isfinite(coef), "balance_loss: coef is not finite");
+  if (mask.has_value() && mask->defined()) {
+    TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == at::kBool && mask->sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                "balance_loss: the mask is bool ", logits.sizes().slice(0, logits.dim() - 1), " on the logits' device");
+  }
+  auto out = BalanceLoss::apply(logits, mask, top_k, coef);
+  return {out[0], out[1], out[2]};
+}
+
 // All blocks' forward filters on the `prep` stream, ahead of the forward pass (see PrepEntry).  w_in[i]: the x extent of
 // block i's input (selects the formulation exactly as mode_conv3d does), need_dx[i]: the block's input needs a gradient.
 void op_prepare_filters(const std::vector<Tensor>& k5, const std::vector<Tensor>& k3, const std::vector<Tensor>& k1,
@@ -2162,6 +2380,12 @@ TORCH_LIBRARY(repmode, m) {
         "float eps, int step) -> ()", &rm::op_adam_step);
   m.def("adam_step_dev(Tensor[] params, Tensor[] grads, Tensor[] exp_avgs, Tensor[] exp_avg_sqs, float lr, float beta1, float beta2, "
         "float eps, Tensor(a!) step_dev, Tensor(b!) hyper_dev) -> ()", &rm::op_adam_step_dev);
+  m.def("grad_norm(Tensor[] tensors, float max_norm) -> (Tensor, Tensor)", &rm::op_grad_norm);
+  m.def("adamw_step(Tensor[] params, Tensor[] grads, Tensor[] exp_avgs, Tensor[] exp_avg_scales, Tensor[] exp_avg_sqs, "
+        "Tensor[] exp_avg_sq_scales, float lr, float beta1, float beta2, float eps, float weight_decay, int step, Tensor? step_dev, "
+        "Tensor? lr_dev, Tensor? clip, int seed) -> ()", &rm::op_adamw_step);
+  m.def("graph_alive(Tensor[] leaves) -> bool", &rm::op_graph_alive);
+  m.def("balance_loss(Tensor logits, Tensor? mask, int top_k, float coef) -> (Tensor, Tensor, Tensor)", &rm::op_balance_loss);
   m.def("clear_frag_store() -> ()", &rm::op_clear_frag_store);
   m.def("pinned_operands() -> Tensor[]", &rm::op_pinned_operands);
   m.def("set_frag_store(bool on) -> ()", &rm::op_set_frag_store);

@@ -56,7 +56,18 @@ def patch_grid(img_size, patch_size, overlap=0.5):
 
 class Model(object):
     def __init__(self, opts, nn_module='RepMode', init_weights=True, lr=0.001, criterion_fn=torch.nn.MSELoss,
-                 gpu_ids=0, mult_chan=32, dtype=torch.bfloat16, distributed=False, hip_graph=False, grad_compress=None):
+                 gpu_ids=0, mult_chan=32, dtype=torch.bfloat16, distributed=False, hip_graph=False, grad_compress=None,
+                 optimizer='adam', optimizer_args=None, balance_coef=0.0):
+        # optimizer: 'adam' (the reference's) or 'adamw' (optim.AdamW: weight decay, clipping by the gradients' norm, moments in 8
+        # bits; optimizer_args goes to its constructor).  balance_coef > 0 adds Net.gate_balance's term to the loss.
+        if optimizer not in ('adam', 'adamw'):
+            raise ValueError("optimizer must be 'adam' or 'adamw', got %r" % (optimizer,))
+        if optimizer == 'adam' and optimizer_args:
+            raise ValueError('optimizer_args go with optimizer=\'adamw\': the reference trains with plain Adam')
+        if not balance_coef >= 0:
+            raise ValueError('balance_coef must not be negative, got %r' % (balance_coef,))
+        self.optimizer_name, self.optimizer_args, self.balance_coef = optimizer, dict(optimizer_args or {}), float(balance_coef)
+        self.last_balance = None
         self.opts = opts
         self.nn_module = nn_module
         self.lr = lr
@@ -126,9 +137,13 @@ class Model(object):
         # version counter and no optimizer hook to say so: with the STOCK optimizer a model that replays its step lays the
         # per-expert blocks' operands out at every forward pass (store off); with the build's own optimizer the captured pass
         # writes the stored operands itself, replay after replay (repmode_ops.cpp op_prepare_filters)
-        own_adam = os.environ.get('REPMODE_ADAM', '1') != '0'
+        own_adam = self.optimizer_name == 'adam' and os.environ.get('REPMODE_ADAM', '1') != '0'
         ops_.torch_ops().set_frag_store((own_adam or not self.hip_graph) and os.environ.get('REPMODE_FRAG_STORE', '1') != '0')
-        if not own_adam:
+        if self.optimizer_name == 'adamw':
+            # (writes no expert operands: as with a stock optimizer, the next forward pass lays them out)
+            from .optim import AdamW
+            self.optimizer = AdamW(self.net.parameters(), lr=self.lr, capturable=self.hip_graph, **self.optimizer_args)
+        elif not own_adam:
             # (REPMODE_ADAM=0: the stock fused optimizer, for A/B; capturable: its step counters live on the device)
             self.optimizer = torch.optim.Adam(self.net.parameters(), lr=self.lr, fused=True, capturable=self.hip_graph)
         else:
@@ -200,7 +215,13 @@ class Model(object):
         if measure:
             ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
             ev[0].record()
-        loss.backward()
+        if self.balance_coef:
+            # (the logged loss stays the criterion's; the term and the counts are in last_balance)
+            balance, counts, _ = self.net.gate_balance(plan, self.balance_coef)
+            self.last_balance = (balance.detach(), counts)
+            (loss + balance).backward()
+        else:
+            loss.backward()
         if measure:
             ev[1].record()
             self._bwd_events.append(ev)
@@ -313,6 +334,9 @@ class Model(object):
                     out = self._train_step(signal, target, ops_.TaskPlan(host, self.net.num_tasks, self.device, True))
                 cur.wait_stream(cs)
                 return out
+            if ops_.torch_ops().graph_alive(list(self.net.parameters())):
+                raise RuntimeError('Model(hip_graph=True): an autograd graph of the network is alive (an output or a gate_balance loss '
+                                   'that was computed with gradients and is still held): release it before a step is captured')
             st['signal'], st['target'] = signal.clone(), target.clone()
             st['plan'] = ops_.TaskPlan(host, self.net.num_tasks, self.device, True)
             graph = torch.cuda.CUDAGraph()
@@ -328,6 +352,7 @@ class Model(object):
             # (the store may drop its entries -- another optimizer steps, another Model is built -- while replays go on)
             st['operands'] = ops_.torch_ops().pinned_operands()
             st['log'] = self._last_log[:4]
+            st['balance'], st['norm'] = self.last_balance, getattr(self.optimizer, 'last_norm', None)
             st['plan'].bn_counted = False
         else:
             st['signal'].copy_(signal, non_blocking=True)
@@ -340,7 +365,9 @@ class Model(object):
             sp.sample_task.copy_(new.sample_task, non_blocking=True)
             sp.tasks_host, sp.slot_task_host = new.tasks_host, new.slot_task_host
         st['graph'].replay()
-        self.last_loss = st['last_loss']
+        self.last_loss, self.last_balance = st['last_loss'], st['balance']
+        if st['norm'] is not None:
+            self.optimizer.last_norm = st['norm']
         self._last_log = st['log'] + (host,)
         return st['out']
 

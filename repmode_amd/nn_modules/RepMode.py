@@ -233,6 +233,26 @@ class Net(torch.nn.Module):
             ops.torch_ops().finish_prepared(y)
         return y
 
+    def gate_balance(self, t, coef=1.0, top_k=1):
+        """``(loss, counts, prob)`` of the network's gates for the tasks ``t`` (ints, one-hot rows or a ``TaskPlan``): the balance loss
+        (``ops.balance_loss``) over the experts of every MoDE block, averaged over the blocks -- a block's rows are its output
+        channels for each sample's task, so the term is ``coef`` where the filters use their experts alike and grows as they settle
+        on few -- and, [blocks, experts], how many of a block's rows prefer each expert and the experts' mean gate values.  The
+        gradient reaches every gate's weight and bias."""
+        device = self.conv_out.gate.weight.device
+        plan = t if isinstance(t, ops.TaskPlan) else ops.TaskPlan(t, self.num_tasks, device, self.training)
+        onehot = (torch.arange(self.num_tasks, device=device)[:, None] == plan.sample_task[None]).to(torch.float32)    # [tasks, samples]
+        losses, counts, probs = [], [], []
+        for m in self.modules():
+            if isinstance(m, MoDEConv):
+                # (experts the slowest axis, as the gate lays them out: RepMode.py:198-200)
+                logits = torch.addmm(m.gate.bias[:, None], m.gate.weight, onehot).view(NUM_EXPERTS, -1).t()
+                loss, count, prob = ops.balance_loss(logits, top_k, coef=coef)
+                losses.append(loss)
+                counts.append(count)
+                probs.append(prob)
+        return torch.stack(losses).mean(), torch.stack(counts), torch.stack(probs)
+
     def _prepare_filters(self, x, plan):
         """The forward filters of all 19 MoDE blocks depend on the parameters and the batch's tasks only: their gate softmax +
         GatRep (or expert layout) launches are issued now, on the library's preparation stream, and run beside the first

@@ -376,6 +376,63 @@ def adam_expert_frags(k5s, k3s, lr, beta1, beta2, eps, step, want_wd=True):
     return outs
 
 
+ADAMW_BLOCK = 256       # elements that share a power of two in the 8-bit moments (REPMODE_ADAMW_BLOCK)
+
+
+def grad_norm(tensors, max_norm=None):
+    """``(norm, clip)``: the 2-norm of all ``tensors`` together (float32 or bfloat16, any strides; sums in float64, in a fixed
+    order) and the factor ``min(1, max_norm / (norm + 1e-6))`` that clips them, both float32 scalars on the device -- no
+    synchronisation, nothing is scaled here.  ``clip`` is NaN where the norm is not finite (``adamw_step`` then leaves the
+    step out); without ``max_norm`` it is 1.  No autograd."""
+    return torch_ops().grad_norm(list(tensors), float('inf') if max_norm is None else float(max_norm))
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, clip=None, seed=0):
+    """AdamW's update (decoupled weight decay) of a list of tensors, in place, moments in float32 (csrc/adamw.hip).
+
+    ``params`` / ``grads``: float32 or bfloat16, dense; ``exp_avgs`` / ``exp_avg_sqs``: float32 of the same shapes and strides.
+    bfloat16 parameters are updated in float32 and rounded once, stochastically, by bits that follow from ``(seed, step, position
+    in the list, element)``.  ``step``: the 1-based count of this update, or an int64 tensor of one value on the device that the
+    call itself advances (a step that is captured into a graph; ``lr`` may then be a float32 tensor of one value too).
+    ``clip``: a float32 device scalar that multiplies the gradients (``grad_norm``); NaN leaves everything as it is."""
+    adamw8_step(params, grads, exp_avgs, [], exp_avg_sqs, [], step, lr, betas, eps, weight_decay, clip, seed)
+
+
+def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+                weight_decay=1e-2, clip=None, seed=0):
+    """``adamw_step`` with the moments in 8 bits: ``exp_avgs`` float8_e4m3fn and ``exp_avg_sqs`` float8_e5m2 of the parameters' shapes
+    and strides, each times the power of two (float8_e8m0fnu) of its block of 256 elements in memory order
+    (``adamw8_state`` makes them).  The arithmetic is float32; what is kept is rounded stochastically.  A tensor whose moments
+    are float32 is updated as ``adamw_step`` does (its scales are not looked at): one list may hold both kinds."""
+    on_device, lr_on_device = torch.is_tensor(step), torch.is_tensor(lr)
+    torch_ops().adamw_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, 0.0 if lr_on_device else float(lr),
+                           float(betas[0]), float(betas[1]), float(eps), float(weight_decay), 0 if on_device else int(step),
+                           step if on_device else None, lr if lr_on_device else None, clip, int(seed))
+
+
+def adamw8_state(param):
+    """Zero moments for ``adamw8_step``: ``(exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale)``."""
+    blocks = -(-param.numel() // ADAMW_BLOCK)
+    zero = lambda dtype: torch.zeros_like(param, dtype=torch.uint8).view(dtype)
+    scale = lambda: torch.full((blocks,), 127, dtype=torch.uint8, device=param.device).view(torch.float8_e8m0fnu)
+    return zero(torch.float8_e4m3fn), scale(), zero(torch.float8_e5m2), scale()
+
+
+def balance_loss(logits, top_k, mask=None, coef=1.0):
+    """The load-balance loss of a router or of a mixture's gates (csrc/balance.hip): ``(loss, counts, prob)``.
+
+    ``logits``: [rows, experts] or [groups, rows, experts] (each group is balanced by itself), float32 or bfloat16, any strides, up
+    to 1024 experts.  With p = softmax(logits) and each row's ``top_k`` largest experts chosen (ties: the lowest index first; an
+    expert at -inf never), f the share of a group's choices that go to an expert and P the mean of its p,
+
+        loss = coef * experts * mean over the groups that have rows of sum_e f_e P_e        (coef, where all are used alike)
+
+    ``mask``: bool, False = the row does not count and is not read (padding).  ``counts`` (int64) and ``prob`` (float32), [experts]
+    or [groups, experts]: the choices of each expert and its mean probability.  The loss's gradient reaches the logits through p;
+    counts and prob carry none.  A NaN in a row that counts makes the loss NaN."""
+    return torch_ops().balance_loss(logits, mask, int(top_k), float(coef))
+
+
 def gate_softmax_samples(gate_w, gate_b, plan, co):
     """g[n, e, o] per SAMPLE (the same kernel with one "slot" per sample)."""
     g = torch.empty((plan.n, NUM_EXPERTS, co), dtype=torch.float32, device=gate_w.device)

@@ -7,6 +7,9 @@ checkpoints, fnet_model.py:57-65); only ``step()`` differs: one call into the op
 parameter with two kernel families and -- for the 5x5x5 / 3x3x3 experts of the blocks that run the per-expert formulation --
 emits the updated experts as the convolution kernels' bf16 operands in the same pass (``repmode_adam_expert_frags``), so the
 next forward pass has no layout launch.  No CPU path: parameters must live on the HIP device.
+
+``AdamW`` is for what the reference does not train with: decoupled weight decay, clipping by the gradients' common norm, bfloat16
+parameters and moments in 8 bits.
 """
 import torch
 
@@ -121,4 +124,144 @@ class Adam(torch.optim.Adam):
                 sel = (lambda xs: xs) if len(idx) == len(params) else (lambda xs: [xs[i] for i in idx])
                 ops_.torch_ops().adam_step(sel(params), sel(grads), sel(exp_avgs), sel(exp_avg_sqs), lr, float(beta1), float(beta2),
                                            float(group['eps']), t)
+        return loss
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) over all tensors at once, with the gradients clipped by their common norm in the same step
+    and the moments in float32 or in 8 bits (csrc/adamw.hip, csrc/grad_norm.hip).  float32 and bfloat16 parameters.
+
+    ``max_norm``: the gradients of all groups together are scaled by ``min(1, max_norm / (norm + 1e-6))`` on their way into the
+    update (``.grad`` itself stays as it is; ``last_norm`` is the norm, a device scalar).  Where the norm is not finite the step
+    changes no parameter and no moment.
+    ``state_bits``: 32, or 8 -- e4m3 / e5m2 values with a power of two for each 256 elements, rounded stochastically: 2 bytes a
+    parameter instead of 8.  Tensors of fewer than ``min_8bit_numel`` elements (biases, norms) keep float32 moments.  Both may be
+    set per group.
+    ``seed``: of the stochastic roundings (8-bit moments, bfloat16 parameters); a run with the same seed repeats itself.
+    ``capturable``: the step count of each group lives on the device, so that ``step()`` can be part of a captured HIP graph (after
+    one step launch by launch); a group's ``lr`` may then be a float32 tensor of one value on the device, which replays read.
+
+    The state of a float32 parameter with 32-bit moments is ``torch.optim.AdamW``'s (``step``, ``exp_avg``, ``exp_avg_sq``): their state
+    dicts interchange.  Loaded moments keep the bits they were saved with.  No CPU path."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None, state_bits=32, min_8bit_numel=4096,
+                 capturable=False, seed=0):
+        if not (torch.is_tensor(lr) or lr >= 0) or not eps >= 0 or not weight_decay >= 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError('repmode_amd.optim.AdamW: bad hyper-parameters')
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError('repmode_amd.optim.AdamW: max_norm must be positive, got %r' % (max_norm,))
+        self.max_norm, self.seed, self.device_step, self.last_norm = max_norm, int(seed), bool(capturable), None
+        self._step_dev = {}          # group index -> int64[1] on the device (capturable)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      min_8bit_numel=min_8bit_numel))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        if self.param_groups[-1]['state_bits'] not in (8, 32):
+            bits = self.param_groups.pop()['state_bits']
+            raise ValueError('repmode_amd.optim.AdamW: moments in 8 or 32 bits, got %r' % (bits,))
+
+    def _state(self, p, group):
+        st = self.state[p]
+        if not st:
+            from . import ops as ops_
+            st['step'] = torch.tensor(0.0)
+            if group['state_bits'] == 8 and p.numel() >= group['min_8bit_numel']:
+                st['exp_avg'], st['exp_avg_scale'], st['exp_avg_sq'], st['exp_avg_sq_scale'] = ops_.adamw8_state(p)
+            else:
+                st['exp_avg'] = torch.zeros_like(p, dtype=torch.float32)
+                st['exp_avg_sq'] = torch.zeros_like(p, dtype=torch.float32)
+        return st
+
+    def sync_steps(self):
+        """Device step counts -> the host counters of ``state`` (after graph replays, which run no host code).  One read a group."""
+        for gi, dev in self._step_dev.items():
+            t = float(dev.item())
+            for p in self.param_groups[gi]['params']:
+                if 'step' in self.state.get(p, {}):
+                    self.state[p]['step'] = torch.tensor(t)
+
+    def state_dict(self):
+        self.sync_steps()
+        return super().state_dict()
+
+    def load_state_dict(self, state_dict):
+        own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel')} for g in self.param_groups]
+        super().load_state_dict(state_dict)
+        for group, mine in zip(self.param_groups, own):          # (a stock optimizer's groups have neither)
+            for k, v in mine.items():
+                group.setdefault(k, v)
+        # (the base class casts floating moments to the parameter's type: 8-bit codes and the float32 moments of bfloat16
+        # parameters are taken from the dict as they are)
+        for saved, group in zip(state_dict['param_groups'], self.param_groups):
+            for key, p in zip(saved['params'], group['params']):
+                for k, v in state_dict['state'].get(key, {}).items():
+                    if k == 'step':
+                        self.state[p][k] = torch.tensor(float(v))
+                    elif torch.is_tensor(v):
+                        v = v.detach().to(p.device, copy=True)
+                        self.state[p][k] = v.float() if v.dtype in (torch.bfloat16, torch.float16) else v
+        for gi, dev in list(self._step_dev.items()):             # (captured steps hold the counts by address: in place)
+            counts = {int(self.state[p]['step']) for p in self.param_groups[gi]['params'] if 'step' in self.state.get(p, {})}
+            if len(counts) <= 1:
+                dev.fill_(counts.pop() if counts else 0)
+            else:
+                del self._step_dev[gi]
+
+    def _count_on_device(self, gi, steps, device):
+        """The group's step count on the device; ``steps``: its parameters' host counters, which go on as well."""
+        if gi not in self._step_dev:
+            t0 = {int(s) for s in steps}
+            if len(t0) != 1:
+                raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): the parameters of a group must have seen the same number of steps')
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): run one step launch by launch before capturing')
+            self._step_dev[gi] = torch.full((1,), t0.pop(), dtype=torch.int64, device=device)
+        for s in steps:
+            s += 1
+        return self._step_dev[gi]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from . import ops as ops_
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work, grads = [], []
+        for gi, group in enumerate(self.param_groups):
+            if group.get('amsgrad', False) or group.get('maximize', False):
+                raise RuntimeError('repmode_amd.optim.AdamW: no amsgrad, no maximize')
+            ps = [p for p in group['params'] if p.grad is not None]
+            if any(p.grad.is_sparse for p in ps):
+                raise RuntimeError('repmode_amd.optim.AdamW: dense gradients only')
+            if ps:
+                work.append((gi, group, ps))
+                grads += [p.grad for p in ps]
+        if not work:
+            return loss
+        clip = None
+        if self.max_norm is not None:
+            self.last_norm, clip = ops_.grad_norm(grads, self.max_norm)
+        none = torch.empty(0)
+        for gi, group, ps in work:
+            states = [self._state(p, group) for p in ps]
+            if self.device_step:
+                calls = [(self._count_on_device(gi, [st['step'] for st in states], ps[0].device), range(len(ps)))]
+            else:
+                # parameters that have seen the same number of updates go together (normally: all of them)
+                if torch.is_tensor(group['lr']):
+                    raise RuntimeError('repmode_amd.optim.AdamW: a learning rate on the device needs capturable=True')
+                by_step = {}
+                for i, st in enumerate(states):
+                    st['step'] += 1
+                    by_step.setdefault(int(st['step']), []).append(i)
+                calls = by_step.items()
+            for count, idx in calls:
+                eight = any('exp_avg_scale' in states[i] for i in idx)
+                scales = (lambda k: [states[i].get(k, none) for i in idx]) if eight else (lambda k: [])
+                ops_.adamw8_step([ps[i] for i in idx], [ps[i].grad for i in idx], [states[i]['exp_avg'] for i in idx], scales('exp_avg_scale'),
+                                 [states[i]['exp_avg_sq'] for i in idx], scales('exp_avg_sq_scale'), count, lr=group['lr'],
+                                 betas=group['betas'], eps=group['eps'], weight_decay=group['weight_decay'], clip=clip,
+                                 seed=(gi << 32) + (self.seed & 0xffffffff))
         return loss
