@@ -208,14 +208,17 @@ __global__ __launch_bounds__(256) void patch_blend_kernel(PatchArgs a, const T* 
   for (int n = 0; n < a.nb; ++n) {
     const int lz = z - a.start[n][0], ly = y - a.start[n][1], lx = x - a.start[n][2];
     if ((unsigned)lz < (unsigned)a.pd && (unsigned)ly < (unsigned)a.ph && (unsigned)lx < (unsigned)a.pw) {
+      // (one rounding for the product and one for the sum: the compiler must not join them)
+#pragma clang fp contract(off)
       if (!hit) { ps = pred_sum[at]; ws = weight_sum[at]; hit = true; }
       const size_t li = ((size_t)lz * a.ph + ly) * a.pw + lx;
       const float g = gauss[li];
       float o;
       if constexpr (sizeof(T) == 2) o = bf16_to_f32(out[(size_t)n * a.pd * a.ph * a.pw + li]);
       else o = out[(size_t)n * a.pd * a.ph * a.pw + li];
-      ps = __fadd_rn(ps, __fmul_rn(o, g));
-      ws = __fadd_rn(ws, g);
+      const float og = o * g;
+      ps = ps + og;
+      ws = ws + g;
     }
   }
   if (hit) { pred_sum[at] = ps; weight_sum[at] = ws; }
