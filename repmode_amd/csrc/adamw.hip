@@ -36,7 +36,7 @@ struct AdamWHyper {
   float w1;          // 1 - beta1
   float beta2;
   float w2;          // 1 - beta2
-  float bc2_sqrt;    // sqrt(1 - beta2^t)
+  float root;        // 1 / sqrt(1 - beta2^t)
   float eps;
   float step;        // lr / (1 - beta1^t)
   float decay;       // 1 - lr * weight_decay
@@ -72,35 +72,40 @@ struct AdamWArgs {
 };
 static_assert(sizeof(AdamWArgs) <= 4096, "launch arguments");
 
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, bool vec, long left) {
+// ---- four elements of a lane.  WHOLE: all of them lie in the tensor and the address suits one access
+template <bool WHOLE>
+__device__ __forceinline__ f32x4 load4(const float* p, int left) {
+  if constexpr (WHOLE) return *reinterpret_cast<const f32x4*>(p);
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (vec && left >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      r = *reinterpret_cast<const f32x4*>(p);
-    } else {
-      const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-      r = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
-    }
-  } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (k < left) r[k] = to_f32<T>(p[k]);
-  }
+  for (int k = 0; k < 4; ++k)
+    if (k < left) r[k] = p[k];
   return r;
 }
-
-__device__ __forceinline__ uint32_t load4_bytes(const uint8_t* p, bool vec, long left) {
-  if (vec && left >= 4) return *reinterpret_cast<const uint32_t*>(p);
+template <bool WHOLE>
+__device__ __forceinline__ f32x4 load4(const bf16_t* p, int left) {
+  if constexpr (WHOLE) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+    return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+  }
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (k < left) r[k] = bf16_to_f32(p[k]);
+  return r;
+}
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t load4(const uint8_t* p, int left) {
+  if constexpr (WHOLE) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t r = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < left) r |= (uint32_t)p[k] << (8 * k);
   return r;
 }
-
-__device__ __forceinline__ void store4(float* p, const f32x4& x, bool vec, long left) {
-  if (vec && left >= 4) {
+template <bool WHOLE>
+__device__ __forceinline__ void store4(float* p, const f32x4& x, int left) {
+  if constexpr (WHOLE) {
     *reinterpret_cast<f32x4*>(p) = x;
     return;
   }
@@ -108,9 +113,9 @@ __device__ __forceinline__ void store4(float* p, const f32x4& x, bool vec, long 
   for (int k = 0; k < 4; ++k)
     if (k < left) p[k] = x[k];
 }
-
-__device__ __forceinline__ void store4_bytes(uint8_t* p, uint32_t x, bool vec, long left) {
-  if (vec && left >= 4) {
+template <bool WHOLE>
+__device__ __forceinline__ void store4(uint8_t* p, uint32_t x, int left) {
+  if constexpr (WHOLE) {
     *reinterpret_cast<uint32_t*>(p) = x;
     return;
   }
@@ -119,36 +124,71 @@ __device__ __forceinline__ void store4_bytes(uint8_t* p, uint32_t x, bool vec, l
     if (k < left) p[k] = (uint8_t)(x >> (8 * k));
 }
 
-// float32 -> bfloat16, up with the probability of the 16 bits cut off
-__device__ __forceinline__ bf16_t round_param(float x, uint32_t bits16) {
-  uint32_t u = __float_as_uint(x);
-  if ((u & 0x7f800000u) != 0x7f800000u) u += bits16;
-  else if (u & 0x7fffffu) u |= 0x400000u;
-  return (bf16_t)(u >> 16);
-}
-
-__device__ __forceinline__ void store4_param(float* p, const f32x4& x, bool vec, long left, uint32_t, uint32_t) { store4(p, x, vec, left); }
-__device__ __forceinline__ void store4_param(bf16_t* p, const f32x4& x, bool vec, long left, uint32_t key, uint32_t index) {
-  bf16_t r[4];
+// The random bits mix32(index ^ key) of a lane's four elements, j = 0, 4, .. of a chunk that starts at a multiple of AW_CHUNK (a power
+// of two below 2^16).  There the first round's x ^ (x >> 16) is s ^ j with one s for the whole chunk, and its product
+// with the odd factor differs between the four elements by multiples of that factor which are the chunk's too: one multiplication
+// instead of four.
+struct Noise {
+  uint32_t s, c[4];
+  __device__ __forceinline__ Noise(uint32_t chunk, uint32_t key) {
+    const uint32_t x = chunk ^ key, t = x ^ (x >> 16);
+    s = t & ~3u;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) r[k] = round_param(x[k], mix32((index + k) ^ key) & 0xffffu);
-  if (vec && left >= 4) {
-    *reinterpret_cast<u32x2*>(p) = u32x2{(uint32_t)r[0] | ((uint32_t)r[1] << 16), (uint32_t)r[2] | ((uint32_t)r[3] << 16)};
+    for (int k = 0; k < 4; ++k) c[k] = ((t & 3u) ^ k) * 0x455c2ed3u;
+  }
+  __device__ __forceinline__ void operator()(uint32_t j, uint32_t (&h)[4]) const {
+    const uint32_t product = (s ^ j) * 0x455c2ed3u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t z = product + c[k];
+      z = (z ^ (z >> 15)) * 0x55a35cd1u;
+      h[k] = z ^ (z >> 16);
+    }
+  }
+};
+static_assert((AW_CHUNK & (AW_CHUNK - 1)) == 0 && AW_CHUNK <= (1 << 16), "Noise");
+
+// parameters: float32 as they are; bfloat16 up with the probability of the 16 bits cut off
+template <bool WHOLE>
+__device__ __forceinline__ void store4_param(float* p, const f32x4& x, int left, const Noise&, uint32_t) { store4<WHOLE>(p, x, left); }
+template <bool WHOLE>
+__device__ __forceinline__ void store4_param(bf16_t* p, const f32x4& x, int left, const Noise& noise, uint32_t j) {
+  uint32_t h[4], r[4];
+  noise(j, h);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)                                  // (a NaN's bits must not run over into the sign)
+    r[k] = x[k] == x[k] ? __float_as_uint(x[k]) + (h[k] & 0xffffu) : 0x7fc00000u;
+  if constexpr (WHOLE) {
+    *reinterpret_cast<u32x2*>(p) = u32x2{(r[0] >> 16) | (r[1] & 0xffff0000u), (r[2] >> 16) | (r[3] & 0xffff0000u)};
     return;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (k < left) p[k] = r[k];
+    if (k < left) p[k] = (bf16_t)(r[k] >> 16);
 }
 
-__device__ __forceinline__ void update(const AdamWHyper& h, float clip, f32x4& p, const f32x4& grad, f32x4& m, f32x4& v) {
+// m, v: one rounding per operation.  p: square root and reciprocal of the hardware (1 ulp each; they take numbers below 2^-126 for zero,
+// so such a v goes through a square root of 2^100 v).
+__device__ __forceinline__ void update(const AdamWHyper& h, float clip, f32x4& p, const f32x4& grad, f32x4& m, f32x4& v, float v_scale) {
+  const float b = h.beta2 * v_scale;
+  uint32_t least = ~0u;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float g = grad[k] * clip;
     m[k] = m[k] + h.w1 * (g - m[k]);
-    v[k] = v[k] * h.beta2 + h.w2 * g * g;
-    p[k] = p[k] * h.decay - h.step * (m[k] / (sqrtf(v[k]) / h.bc2_sqrt + h.eps));
+    v[k] = v[k] * b + h.w2 * g * g;
+    const uint32_t u = __float_as_uint(v[k]) - 1u;            // (zero: the largest)
+    least = u < least ? u : least;
   }
+  f32x4 root;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) root[k] = __builtin_amdgcn_sqrtf(v[k]);
+  if (least < 0x0d800000u) {                                   // 2^-100
+#pragma unroll
+    for (int k = 0; k < 4; ++k) root[k] = v[k] < 0x1p-100f ? __builtin_amdgcn_sqrtf(v[k] * 0x1p100f) * 0x1p-50f : root[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) p[k] = fmaf(-(h.step * m[k]), __builtin_amdgcn_rcpf(fmaf(root[k], h.root, h.eps)), p[k] * h.decay);
 }
 
 // the values of 4 e4m3 / e5m2 codes
@@ -162,34 +202,138 @@ __device__ __forceinline__ f32x4 decode_e5m2(uint32_t w) {
 }
 __device__ __forceinline__ float power_of_two(uint32_t biased) { return __uint_as_float(biased << 23); }      // 2^(biased - 127), 1..254
 
-// The largest finite magnitude's biased exponent over the wave's 256 elements, less `room`, at least 1: the block's power of two.
-__device__ __forceinline__ uint32_t block_scale(const f32x4& x, int room) {
+// the largest over the wave, in a scalar register: rows of 16 lanes by shifts, then the rows by two broadcasts
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  auto step = [&](uint32_t o) { x = o > x ? o : x; };
+  step(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));      // row_shr:1
+  step(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+  step(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));     // row_bcast:15 into rows 1 and 3
+  step(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));     // row_bcast:31 into rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ uint32_t largest(const f32x4& x, uint32_t below) {      // of the bits of |x| that are less than `below`
   uint32_t most = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const uint32_t u = __float_as_uint(x[k]) & 0x7fffffffu;
-    if (u < 0x7f800000u && u > most) most = u;
+    most = u > most && u < below ? u : most;
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)most, off, 64);
-    if (o > most) most = o;
-  }
+  return wave_max(most);
+}
+// the block's power of two (biased): brings its largest magnitude to [2^room, 2^(room + 1))
+__device__ __forceinline__ uint32_t block_power(uint32_t most, int room) {
   const int e = (int)(most >> 23) - room;
   return (uint32_t)(e < 1 ? 1 : e);
 }
 
-// A magnitude x (already times the block's inverse power) as the code of a float with MAN mantissa bits and bias BIAS: `up`, of
-// the 23 - MAN bits that are cut off, is added before the cut.  Below the smallest normal value the steps stay as they are
-// there: adding that value puts them at the same place of the float32 mantissa.
-template <int MAN, int BIAS, uint32_t INF, uint32_t NAN_>
-__device__ __forceinline__ uint32_t encode(float x, uint32_t up) {
-  const float least = __uint_as_float((uint32_t)(128 - BIAS) << 23);
-  const bool low = x < least;
-  const uint32_t u = __float_as_uint(low ? x + least : x);
-  const uint32_t code = ((u + up) >> (23 - MAN)) - (low ? (uint32_t)(128 - BIAS) << MAN : (uint32_t)(127 - BIAS) << MAN);
-  if ((u & 0x7f800000u) == 0x7f800000u) return (u & 0x7fffffu) ? NAN_ : INF;
-  return code;
+// What is not finite, among values that may be: NaN for NaN (and for infinity in e4m3, which has none), infinity in e5m2.
+__device__ __forceinline__ uint32_t encode_special(float x, uint32_t code, bool e5m2) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  if (u < 0x7f800000u) return code;
+  return (__float_as_uint(x) >> 24 & 0x80u) | (!e5m2 ? 0x7fu : u > 0x7f800000u ? 0x7eu : 0x7cu);
+}
+
+// A block's m and v as codes.  The conversions round stochastically by adding the upper 20 (e4m3) or 21 (e5m2) bits of their second
+// operand to the part cut off -- also below the smallest normal value -- which is this file's rounding with 16 random bits and a half.
+__device__ __forceinline__ void encode4(const f32x4& m, const f32x4& v, const uint32_t (&h)[4], uint32_t& mw, uint32_t& vw, uint32_t& me, uint32_t& ve) {
+  uint32_t most_m = largest(m, ~0u), most_v = largest(v, ~0u);
+  const bool finite = most_m < 0x7f800000u && most_v < 0x7f800000u;           // (of the whole block)
+  if (!finite) { most_m = largest(m, 0x7f800000u); most_v = largest(v, 0x7f800000u); }
+  me = block_power(most_m, 7);
+  ve = block_power(most_v, 14);
+  const float mi = power_of_two(254 - me), vi = power_of_two(254 - ve);
+  float x[4], y[4];
+  uint32_t a[4], b[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = m[k] * mi;
+    y[k] = fmaxf(v[k] * vi, v[k] > 0.f ? 0x1p-16f : 0.f);                     // (above zero: not rounded to zero)
+    a[k] = (h[k] << 16) | 0x8000u;
+    b[k] = (h[k] & 0xffff0000u) | 0x8000u;
+  }
+  int p = 0, q = 0;
+  p = __builtin_amdgcn_cvt_sr_fp8_f32(x[0], a[0], p, 0);
+  p = __builtin_amdgcn_cvt_sr_fp8_f32(x[1], a[1], p, 1);
+  p = __builtin_amdgcn_cvt_sr_fp8_f32(x[2], a[2], p, 2);
+  p = __builtin_amdgcn_cvt_sr_fp8_f32(x[3], a[3], p, 3);
+  q = __builtin_amdgcn_cvt_sr_bf8_f32(y[0], b[0], q, 0);
+  q = __builtin_amdgcn_cvt_sr_bf8_f32(y[1], b[1], q, 1);
+  q = __builtin_amdgcn_cvt_sr_bf8_f32(y[2], b[2], q, 2);
+  q = __builtin_amdgcn_cvt_sr_bf8_f32(y[3], b[3], q, 3);
+  mw = (uint32_t)p;
+  vw = (uint32_t)q;
+  if (!finite) {
+    uint32_t mc = 0, vc = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      mc |= encode_special(m[k], (mw >> (8 * k)) & 0xffu, false) << (8 * k);
+      vc |= encode_special(v[k], (vw >> (8 * k)) & 0xffu, true) << (8 * k);
+    }
+    mw = mc;
+    vw = vc;
+  }
+}
+
+// One workgroup's chunk.  WHOLE: the chunk lies in the tensor and every address suits one access of four elements; all its loads are
+// under way before the first is used.  Otherwise block by block, element by element where that has to be.
+template <typename T, bool EIGHT, bool WHOLE, int UNITS>
+__device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const AdamWHyper& h, float clip, uint32_t key, long chunk, int unit, int wave,
+                                            int lane, long n) {
+  using S = std::conditional_t<EIGHT, uint8_t, float>;
+  using W = std::conditional_t<EIGHT, uint32_t, f32x4>;
+  const Noise state_noise((uint32_t)chunk, key), param_noise((uint32_t)chunk, mix32(key ^ AW_PARAM_KEY));
+  f32x4 P[UNITS], G[UNITS];
+  W M[UNITS], V[UNITS];
+  uint32_t ME[UNITS], VE[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const long o = chunk + ((unit + u) * AW_WAVES + wave) * AW_BLOCK;         // of the wave's block; uniform
+    const int left = WHOLE ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
+    P[u] = load4<WHOLE>(static_cast<const T*>(a.p[i]) + o + lane * 4, left);
+    G[u] = load4<WHOLE>(static_cast<const T*>(a.g[i]) + o + lane * 4, left);
+    M[u] = load4<WHOLE>(static_cast<const S*>(a.m[i]) + o + lane * 4, left);
+    V[u] = load4<WHOLE>(static_cast<const S*>(a.v[i]) + o + lane * 4, left);
+    if constexpr (EIGHT) {
+      ME[u] = a.ms[i][o / AW_BLOCK];
+      VE[u] = a.vs[i][o / AW_BLOCK];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int j = ((unit + u) * AW_WAVES + wave) * AW_BLOCK + lane * 4;
+    const long o = chunk + ((unit + u) * AW_WAVES + wave) * AW_BLOCK;
+    const int left = WHOLE ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
+    T* p = static_cast<T*>(a.p[i]) + o + lane * 4;
+    S* m = static_cast<S*>(a.m[i]) + o + lane * 4;
+    S* v = static_cast<S*>(a.v[i]) + o + lane * 4;
+    if constexpr (EIGHT) {
+      const uint32_t me0 = __builtin_amdgcn_readfirstlane(ME[u]), ve0 = __builtin_amdgcn_readfirstlane(VE[u]);
+      f32x4 m4 = decode_e4m3(M[u]) * power_of_two(me0), v4 = decode_e5m2(V[u]);
+      update(h, clip, P[u], G[u], m4, v4, power_of_two(ve0));
+      if constexpr (!WHOLE) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k >= left) m4[k] = v4[k] = 0.f;                                  // (behind the tensor's end: not of the block)
+      }
+      uint32_t r[4], mw, vw, me, ve;
+      state_noise(j, r);
+      encode4(m4, v4, r, mw, vw, me, ve);
+      store4_param<WHOLE>(p, P[u], left, param_noise, j);
+      store4<WHOLE>(m, mw, left);
+      store4<WHOLE>(v, vw, left);
+      if (lane == 0) {
+        a.ms[i][o / AW_BLOCK] = (uint8_t)me;
+        a.vs[i][o / AW_BLOCK] = (uint8_t)ve;
+      }
+    } else {
+      update(h, clip, P[u], G[u], M[u], V[u], 1.f);
+      store4_param<WHOLE>(p, P[u], left, param_noise, j);
+      store4<WHOLE>(m, M[u], left);
+      store4<WHOLE>(v, V[u], left);
+    }
+  }
 }
 
 template <typename T, bool EIGHT>
@@ -198,87 +342,29 @@ __global__ __launch_bounds__(64 * AW_WAVES) void adamw_kernel(AdamWArgs a) {
   if (clip != clip) return;                                   // gradients that are not finite: the step is left out
   const AdamWHyper h = a.hd ? *a.hd : a.h;
   int i = 0;
-  for (int lo = 0, hi = a.nt; hi - lo > 1;) {                  // the tensor of this workgroup: first[i] <= blockIdx.x < first[i + 1]
-    const int mid = (lo + hi) >> 1;
-    if ((int)blockIdx.x >= a.first[mid]) lo = mid;
+  for (int hi = a.nt; hi - i > 1;) {                           // the tensor of this workgroup: first[i] <= blockIdx.x < first[i + 1]
+    const int mid = (i + hi) >> 1;
+    if ((int)blockIdx.x >= a.first[mid]) i = mid;
     else hi = mid;
-    i = lo;
   }
   const long n = a.numel[i];
-  T* __restrict__ p = static_cast<T*>(a.p[i]);
-  const T* __restrict__ g = static_cast<const T*>(a.g[i]);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long chunk = (long)((int)blockIdx.x - a.first[i]) * AW_CHUNK;
   // (a chunk never crosses a multiple of 2^32: the upper half of the element index is the workgroup's)
   uint32_t key = mix32(h.base + (uint32_t)a.position[i]);
   if (chunk >> 32) key = mix32(key + (uint32_t)(chunk >> 32));
-  const bool vec_p = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
-  f32x4 P[AW_UNITS], G[AW_UNITS];
-  if constexpr (!EIGHT) {
-    float* __restrict__ m = static_cast<float*>(a.m[i]);
-    float* __restrict__ v = static_cast<float*>(a.v[i]);
-    const bool vec_s = (((uintptr_t)m | (uintptr_t)v) & 15) == 0;
-    f32x4 M[AW_UNITS], V[AW_UNITS];
-#pragma unroll
-    for (int u = 0; u < AW_UNITS; ++u) {
-      const long o = chunk + ((u * AW_WAVES + wave) * 64 + lane) * 4, left = n - o;
-      P[u] = load4(p + o, vec_p, left);
-      G[u] = load4(g + o, vec_p, left);
-      M[u] = load4(m + o, vec_s, left);
-      V[u] = load4(v + o, vec_s, left);
-    }
-#pragma unroll
-    for (int u = 0; u < AW_UNITS; ++u) {
-      const long o = chunk + ((u * AW_WAVES + wave) * 64 + lane) * 4, left = n - o;
-      update(h, clip, P[u], G[u], M[u], V[u]);
-      store4_param(p + o, P[u], vec_p, left, mix32(key ^ AW_PARAM_KEY), (uint32_t)o);
-      store4(m + o, M[u], vec_s, left);
-      store4(v + o, V[u], vec_s, left);
-    }
-  } else {
-    uint8_t* __restrict__ m = static_cast<uint8_t*>(a.m[i]);
-    uint8_t* __restrict__ v = static_cast<uint8_t*>(a.v[i]);
-    uint8_t* __restrict__ ms = a.ms[i];
-    uint8_t* __restrict__ vs = a.vs[i];
-    const bool vec_s = (((uintptr_t)m | (uintptr_t)v) & 3) == 0;
-    uint32_t M8[AW_UNITS], V8[AW_UNITS], ME[AW_UNITS], VE[AW_UNITS];
-#pragma unroll
-    for (int u = 0; u < AW_UNITS; ++u) {
-      const long b = chunk / AW_BLOCK + u * AW_WAVES + wave, o = b * AW_BLOCK + lane * 4, left = n - o;
-      ME[u] = VE[u] = 1;
-      P[u] = load4(p + o, vec_p, left);
-      G[u] = load4(g + o, vec_p, left);
-      M8[u] = load4_bytes(m + o, vec_s, left);
-      V8[u] = load4_bytes(v + o, vec_s, left);
-      if (b * AW_BLOCK < n) { ME[u] = ms[b]; VE[u] = vs[b]; }
-    }
-#pragma unroll
-    for (int u = 0; u < AW_UNITS; ++u) {
-      const long b = chunk / AW_BLOCK + u * AW_WAVES + wave, o = b * AW_BLOCK + lane * 4, left = n - o;
-      if (b * AW_BLOCK >= n) break;                            // (uniform over the wave)
-      f32x4 M = decode_e4m3(M8[u]) * power_of_two(ME[u]), V = decode_e5m2(V8[u]) * power_of_two(VE[u]);
-      update(h, clip, P[u], G[u], M, V);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k >= left) M[k] = V[k] = 0.f;                      // (behind the tensor's end: not of the block)
-      const uint32_t me = block_scale(M, 7), ve = block_scale(V, 14);
-      const float mi = power_of_two(254 - me), vi = power_of_two(254 - ve);
-      uint32_t mw = 0, vw = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t r = mix32(((uint32_t)o + k) ^ key);
-        uint32_t mc = encode<3, 7, 0x7fu, 0x7fu>(fabsf(M[k]) * mi, ((r & 0xffffu) << 4) + 8u);
-        mc |= (__float_as_uint(M[k]) >> 24) & 0x80u;
-        uint32_t vc = encode<2, 15, 0x7cu, 0x7eu>(V[k] * vi, ((r >> 16) << 5) + 16u);
-        if (V[k] > 0.f && vc == 0) vc = 1;
-        mw |= mc << (8 * k);
-        vw |= vc << (8 * k);
-      }
-      store4_param(p + o, P[u], vec_p, left, mix32(key ^ AW_PARAM_KEY), (uint32_t)o);
-      store4_bytes(m + o, mw, vec_s, left);
-      store4_bytes(v + o, vw, vec_s, left);
-      if (lane == 0) { ms[b] = (uint8_t)me; vs[b] = (uint8_t)ve; }
-    }
+  constexpr uintptr_t PA = 4 * sizeof(T) - 1, SA = EIGHT ? 3 : 15;
+  const bool aligned = (((uintptr_t)a.p[i] | (uintptr_t)a.g[i]) & PA) == 0 && (((uintptr_t)a.m[i] | (uintptr_t)a.v[i]) & SA) == 0;
+  if (aligned && chunk + AW_CHUNK <= n) {
+    adamw_units<T, EIGHT, true, AW_UNITS>(a, i, h, clip, key, chunk, 0, wave, lane, n);
+    return;
+  }
+#pragma unroll 1
+  for (int u = 0; u < AW_UNITS; ++u) {
+    const long o = chunk + (u * AW_WAVES + wave) * AW_BLOCK;
+    if (o >= n) break;
+    if (aligned && o + AW_BLOCK <= n) adamw_units<T, EIGHT, true, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
+    else adamw_units<T, EIGHT, false, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
   }
 }
 
@@ -287,6 +373,9 @@ int check_hyper(double lr, double beta1, double beta2, double eps, double weight
                  std::isfinite(eps) && std::isfinite(weight_decay), "adamw: bad hyper-parameters");
   return REPMODE_OK;
 }
+
+// (an eps above zero stays so: the reciprocal takes what is below 2^-126 for zero)
+__host__ __device__ __forceinline__ float float_eps(double eps) { return eps > 0 && eps < 0x1p-126 ? 0x1p-126f : (float)eps; }
 
 // one thread: *step_dev += 1, and the constants of that step in the host path's double arithmetic
 __global__ void adamw_hyper_kernel(long* __restrict__ step_dev, AdamWHyper* __restrict__ out, double lr, const float* __restrict__ lr_dev,
@@ -299,8 +388,8 @@ __global__ void adamw_hyper_kernel(long* __restrict__ step_dev, AdamWHyper* __re
   out->w1 = (float)(1.0 - beta1);
   out->beta2 = (float)beta2;
   out->w2 = (float)(1.0 - beta2);
-  out->bc2_sqrt = (float)sqrt(bc2);
-  out->eps = (float)eps;
+  out->root = (float)(1.0 / sqrt(bc2));
+  out->eps = float_eps(eps);
   out->step = (float)(l / bc1);
   out->decay = (float)(1.0 - l * weight_decay);
   out->base = noise_base(seed, (uint64_t)t);
@@ -340,8 +429,8 @@ extern "C" int repmode_adamw_multi(int ntensors, int dtype, int state_bits, void
     a.h.w1 = (float)(1.0 - beta1);
     a.h.beta2 = (float)beta2;
     a.h.w2 = (float)(1.0 - beta2);
-    a.h.bc2_sqrt = (float)std::sqrt(bc2);
-    a.h.eps = (float)eps;
+    a.h.root = (float)(1.0 / std::sqrt(bc2));
+    a.h.eps = float_eps(eps);
     a.h.step = (float)(lr / bc1);
     a.h.decay = (float)(1.0 - lr * weight_decay);
     a.h.base = noise_base(seed, (uint64_t)step);
