@@ -72,20 +72,29 @@ struct AdamWArgs {
 };
 static_assert(sizeof(AdamWArgs) <= 4096, "launch arguments");
 
-// ---- four elements of a lane.  WHOLE: all of them lie in the tensor and the address suits one access
-template <bool WHOLE>
+// ---- four elements of a lane.  AW_WHOLE: all of them lie in the tensor and the address suits one access, which goes past the
+// caches: nothing but the gradients can be there from what ran before, and what is written is next read a whole pass later
+// (4 / 32 / 128 M float32 parameters, float32 moments: 24.6 / 162 / 640 us, through the caches 32.0 / 184 / 706; right after the norm
+// of the same gradients 20.7 / 144 / 603 and 25.0 / 160 / 663.  Only a list of tens of MB that is updated again and again with nothing
+// in between would gain by the caches: 28.3 and 26.1 at 4 M.)
+enum { AW_PART = 0, AW_WHOLE = 1 };
+template <typename V>
+__device__ __forceinline__ V fetch(const V* p) { return __builtin_nontemporal_load(p); }
+template <typename V>
+__device__ __forceinline__ void put(V* p, const V& x) { __builtin_nontemporal_store(x, p); }
+template <int HOW>
 __device__ __forceinline__ f32x4 load4(const float* p, int left) {
-  if constexpr (WHOLE) return *reinterpret_cast<const f32x4*>(p);
+  if constexpr (HOW != AW_PART) return fetch(reinterpret_cast<const f32x4*>(p));
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < left) r[k] = p[k];
   return r;
 }
-template <bool WHOLE>
+template <int HOW>
 __device__ __forceinline__ f32x4 load4(const bf16_t* p, int left) {
-  if constexpr (WHOLE) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+  if constexpr (HOW != AW_PART) {
+    const u32x2 w = fetch(reinterpret_cast<const u32x2*>(p));
     return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
   }
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
@@ -94,29 +103,29 @@ __device__ __forceinline__ f32x4 load4(const bf16_t* p, int left) {
     if (k < left) r[k] = bf16_to_f32(p[k]);
   return r;
 }
-template <bool WHOLE>
+template <int HOW>
 __device__ __forceinline__ uint32_t load4(const uint8_t* p, int left) {
-  if constexpr (WHOLE) return *reinterpret_cast<const uint32_t*>(p);
+  if constexpr (HOW != AW_PART) return fetch(reinterpret_cast<const uint32_t*>(p));
   uint32_t r = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < left) r |= (uint32_t)p[k] << (8 * k);
   return r;
 }
-template <bool WHOLE>
+template <int HOW>
 __device__ __forceinline__ void store4(float* p, const f32x4& x, int left) {
-  if constexpr (WHOLE) {
-    *reinterpret_cast<f32x4*>(p) = x;
+  if constexpr (HOW != AW_PART) {
+    put(reinterpret_cast<f32x4*>(p), x);
     return;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (k < left) p[k] = x[k];
 }
-template <bool WHOLE>
+template <int HOW>
 __device__ __forceinline__ void store4(uint8_t* p, uint32_t x, int left) {
-  if constexpr (WHOLE) {
-    *reinterpret_cast<uint32_t*>(p) = x;
+  if constexpr (HOW != AW_PART) {
+    put(reinterpret_cast<uint32_t*>(p), x);
     return;
   }
 #pragma unroll
@@ -149,17 +158,17 @@ struct Noise {
 static_assert((AW_CHUNK & (AW_CHUNK - 1)) == 0 && AW_CHUNK <= (1 << 16), "Noise");
 
 // parameters: float32 as they are; bfloat16 up with the probability of the 16 bits cut off
-template <bool WHOLE>
-__device__ __forceinline__ void store4_param(float* p, const f32x4& x, int left, const Noise&, uint32_t) { store4<WHOLE>(p, x, left); }
-template <bool WHOLE>
+template <int HOW>
+__device__ __forceinline__ void store4_param(float* p, const f32x4& x, int left, const Noise&, uint32_t) { store4<HOW>(p, x, left); }
+template <int HOW>
 __device__ __forceinline__ void store4_param(bf16_t* p, const f32x4& x, int left, const Noise& noise, uint32_t j) {
   uint32_t h[4], r[4];
   noise(j, h);
 #pragma unroll
   for (int k = 0; k < 4; ++k)                                  // (a NaN's bits must not run over into the sign)
     r[k] = x[k] == x[k] ? __float_as_uint(x[k]) + (h[k] & 0xffffu) : 0x7fc00000u;
-  if constexpr (WHOLE) {
-    *reinterpret_cast<u32x2*>(p) = u32x2{(r[0] >> 16) | (r[1] & 0xffff0000u), (r[2] >> 16) | (r[3] & 0xffff0000u)};
+  if constexpr (HOW != AW_PART) {
+    put(reinterpret_cast<u32x2*>(p), u32x2{(r[0] >> 16) | (r[1] & 0xffff0000u), (r[2] >> 16) | (r[3] & 0xffff0000u)});
     return;
   }
 #pragma unroll
@@ -276,9 +285,8 @@ __device__ __forceinline__ void encode4(const f32x4& m, const f32x4& v, const ui
   }
 }
 
-// One workgroup's chunk.  WHOLE: the chunk lies in the tensor and every address suits one access of four elements; all its loads are
-// under way before the first is used.  Otherwise block by block, element by element where that has to be.
-template <typename T, bool EIGHT, bool WHOLE, int UNITS>
+// UNITS blocks of each wave; all their loads are under way before the first is used.
+template <typename T, bool EIGHT, int HOW, int UNITS>
 __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const AdamWHyper& h, float clip, uint32_t key, long chunk, int unit, int wave,
                                             int lane, long n) {
   using S = std::conditional_t<EIGHT, uint8_t, float>;
@@ -290,11 +298,11 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     const long o = chunk + ((unit + u) * AW_WAVES + wave) * AW_BLOCK;         // of the wave's block; uniform
-    const int left = WHOLE ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
-    P[u] = load4<WHOLE>(static_cast<const T*>(a.p[i]) + o + lane * 4, left);
-    G[u] = load4<WHOLE>(static_cast<const T*>(a.g[i]) + o + lane * 4, left);
-    M[u] = load4<WHOLE>(static_cast<const S*>(a.m[i]) + o + lane * 4, left);
-    V[u] = load4<WHOLE>(static_cast<const S*>(a.v[i]) + o + lane * 4, left);
+    const int left = HOW != AW_PART ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
+    P[u] = load4<HOW>(static_cast<const T*>(a.p[i]) + o + lane * 4, left);
+    G[u] = load4<HOW>(static_cast<const T*>(a.g[i]) + o + lane * 4, left);
+    M[u] = load4<HOW>(static_cast<const S*>(a.m[i]) + o + lane * 4, left);
+    V[u] = load4<HOW>(static_cast<const S*>(a.v[i]) + o + lane * 4, left);
     if constexpr (EIGHT) {
       ME[u] = a.ms[i][o / AW_BLOCK];
       VE[u] = a.vs[i][o / AW_BLOCK];
@@ -304,7 +312,7 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
   for (int u = 0; u < UNITS; ++u) {
     const int j = ((unit + u) * AW_WAVES + wave) * AW_BLOCK + lane * 4;
     const long o = chunk + ((unit + u) * AW_WAVES + wave) * AW_BLOCK;
-    const int left = WHOLE ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
+    const int left = HOW != AW_PART ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
     T* p = static_cast<T*>(a.p[i]) + o + lane * 4;
     S* m = static_cast<S*>(a.m[i]) + o + lane * 4;
     S* v = static_cast<S*>(a.v[i]) + o + lane * 4;
@@ -312,7 +320,7 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
       const uint32_t me0 = __builtin_amdgcn_readfirstlane(ME[u]), ve0 = __builtin_amdgcn_readfirstlane(VE[u]);
       f32x4 m4 = decode_e4m3(M[u]) * power_of_two(me0), v4 = decode_e5m2(V[u]);
       update(h, clip, P[u], G[u], m4, v4, power_of_two(ve0));
-      if constexpr (!WHOLE) {
+      if constexpr (HOW == AW_PART) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (k >= left) m4[k] = v4[k] = 0.f;                                  // (behind the tensor's end: not of the block)
@@ -320,18 +328,18 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
       uint32_t r[4], mw, vw, me, ve;
       state_noise(j, r);
       encode4(m4, v4, r, mw, vw, me, ve);
-      store4_param<WHOLE>(p, P[u], left, param_noise, j);
-      store4<WHOLE>(m, mw, left);
-      store4<WHOLE>(v, vw, left);
+      store4_param<HOW>(p, P[u], left, param_noise, j);
+      store4<HOW>(m, mw, left);
+      store4<HOW>(v, vw, left);
       if (lane == 0) {
         a.ms[i][o / AW_BLOCK] = (uint8_t)me;
         a.vs[i][o / AW_BLOCK] = (uint8_t)ve;
       }
     } else {
       update(h, clip, P[u], G[u], M[u], V[u], 1.f);
-      store4_param<WHOLE>(p, P[u], left, param_noise, j);
-      store4<WHOLE>(m, M[u], left);
-      store4<WHOLE>(v, V[u], left);
+      store4_param<HOW>(p, P[u], left, param_noise, j);
+      store4<HOW>(m, M[u], left);
+      store4<HOW>(v, V[u], left);
     }
   }
 }
@@ -356,15 +364,15 @@ __global__ __launch_bounds__(64 * AW_WAVES) void adamw_kernel(AdamWArgs a) {
   constexpr uintptr_t PA = 4 * sizeof(T) - 1, SA = EIGHT ? 3 : 15;
   const bool aligned = (((uintptr_t)a.p[i] | (uintptr_t)a.g[i]) & PA) == 0 && (((uintptr_t)a.m[i] | (uintptr_t)a.v[i]) & SA) == 0;
   if (aligned && chunk + AW_CHUNK <= n) {
-    adamw_units<T, EIGHT, true, AW_UNITS>(a, i, h, clip, key, chunk, 0, wave, lane, n);
+    adamw_units<T, EIGHT, AW_WHOLE, AW_UNITS>(a, i, h, clip, key, chunk, 0, wave, lane, n);
     return;
   }
 #pragma unroll 1
   for (int u = 0; u < AW_UNITS; ++u) {
     const long o = chunk + (u * AW_WAVES + wave) * AW_BLOCK;
     if (o >= n) break;
-    if (aligned && o + AW_BLOCK <= n) adamw_units<T, EIGHT, true, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
-    else adamw_units<T, EIGHT, false, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
+    if (aligned && o + AW_BLOCK <= n) adamw_units<T, EIGHT, AW_WHOLE, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
+    else adamw_units<T, EIGHT, AW_PART, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
   }
 }
 
@@ -451,10 +459,11 @@ extern "C" int repmode_adamw_multi(int ntensors, int dtype, int state_bits, void
   a.first[ntensors] = (int)total;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)total), block(64 * AW_WAVES);
-  if (dtype == REPMODE_F32 && !eight) hipLaunchKernelGGL((adamw_kernel<float, false>), grid, block, 0, s, a);
-  else if (dtype == REPMODE_F32) hipLaunchKernelGGL((adamw_kernel<float, true>), grid, block, 0, s, a);
-  else if (!eight) hipLaunchKernelGGL((adamw_kernel<bf16_t, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((adamw_kernel<bf16_t, true>), grid, block, 0, s, a);
+  auto launch = [&](auto t, auto e) {
+    hipLaunchKernelGGL((adamw_kernel<decltype(t), decltype(e)::value>), grid, block, 0, s, a);
+  };
+  if (dtype == REPMODE_F32) eight ? launch(float{}, std::true_type{}) : launch(float{}, std::false_type{});
+  else eight ? launch(bf16_t{}, std::true_type{}) : launch(bf16_t{}, std::false_type{});
   RM_LAUNCH_CHECK("adamw_multi");
   return REPMODE_OK;
 }

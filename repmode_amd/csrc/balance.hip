@@ -9,20 +9,27 @@
 //     dx_ne = up * p_ne (w_ge - sum_j w_gj p_nj),     w_ge = coef E f_ge / (G' N_g).
 //
 // A row's E values live in the registers of LPR lanes, 8 (E > 512: 16) a lane, so a row is read once and softmax, choice and
-// the lane's share of the column sums (probabilities in float32, counts as integers) need no memory.  A workgroup walks many
-// rows and writes one partial per expert; one launch adds the partials of a group's columns in a fixed order in float64, one
-// more makes the loss of them where there are several such workgroups.  No float atomics: a run repeats itself bit by bit.
-// The backward pass reads the logits again and needs nothing of a row but its logits.
-// What bounds it: HBM for the backward pass (one read, one write), the choice's rounds for wide forward passes.
+// the lane's share of the column sums (probabilities in float32, counts as integers) need no memory.
+//   The choice needs no order, only the k-th largest value: each lane sorts its values once (a network), then top_k rounds take the
+// row's largest head and move the list of the lane that holds it up by one; what is at least the last round's value is chosen.
+// The first round's value is the softmax's maximum.  All of it on integers that are ordered as the values are; bfloat16
+// values carry their index in the lower half, so no two are equal; float32 rows where more than top_k values
+// reach the last one (equal values) are chosen again one by one, value and index.
+//   A workgroup walks many rows and writes one partial per expert; one launch adds the partials of a group's columns in a fixed
+// order in float64, one more makes the loss of them; where one workgroup has seen all rows it does both itself.  No float atomics: a
+// run repeats itself bit by bit.  The backward pass reads the logits again and needs nothing of a row but its logits.
+// What bounds it: HBM for the backward pass (one read, one write), the instructions of exponential and choice for forward passes.
 #include "common.h"
 
 #include <cmath>
 
 namespace {
 
-constexpr int BL_WAVES = 4;
+constexpr int BL_WAVES = 8;
 constexpr int BL_MAX_E = REPMODE_BALANCE_MAX_EXPERTS;
-constexpr int BL_FINISH = 256;           // threads of the finish: 64 columns, 4 shares of the partials
+constexpr int BL_FINISH = 256;           // threads of the finish
+constexpr int BL_COLUMNS = 8;            // columns of a workgroup of it; the other threads share the partials
+constexpr int BL_BLOCKS = 512;           // most workgroups of a pass: two to a CU, which registers leave room for
 
 struct BalanceArgs {
   const void* x;
@@ -41,24 +48,102 @@ struct BalanceArgs {
   int* valid;                //          [groups][blocks]
 };
 
-// e^x for x <= 0, NaN and -inf: 2^t with t = x log2(e) in two parts (t's rounding alone would cost |x| 2^-24 of the result)
-__device__ __forceinline__ float exp_neg(float x) {
-  const float t = x * 1.44269504f, lo = fmaf(x, 1.44269504f, -t) + x * 1.92596303e-8f;
-  const float r = __builtin_amdgcn_exp2f(t);
-  return x < -104.f ? 0.f : fmaf(r, lo * 0.693147181f, r);
+// ---- over the LPR neighbouring lanes of a row, the result in each of them.  Up to 16 lanes by DPP (inside a row of 16: quads, then
+// mirrors, which do because the quads' lanes agree by then), rows and halves by swaps.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true); }
+template <int LPR, typename T, typename Op>
+__device__ __forceinline__ T over_row(T v, Op op) {
+  auto with = [&](uint32_t o) { v = op(v, __builtin_bit_cast(T, o)); };
+  auto bits = [&]() { return __builtin_bit_cast(uint32_t, v); };
+  if constexpr (LPR >= 2) with(dpp<0xB1>(bits()));          // quad_perm 1 0 3 2
+  if constexpr (LPR >= 4) with(dpp<0x4E>(bits()));          // quad_perm 2 3 0 1
+  if constexpr (LPR >= 8) with(dpp<0x141>(bits()));         // row_half_mirror
+  if constexpr (LPR >= 16) with(dpp<0x140>(bits()));        // row_mirror
+  if constexpr (LPR >= 32) {
+    const auto w = __builtin_amdgcn_permlane16_swap(bits(), bits(), false, false);
+    v = op(__builtin_bit_cast(T, (uint32_t)w[0]), __builtin_bit_cast(T, (uint32_t)w[1]));
+  }
+  if constexpr (LPR >= 64) {
+    const auto w = __builtin_amdgcn_permlane32_swap(bits(), bits(), false, false);
+    v = op(__builtin_bit_cast(T, (uint32_t)w[0]), __builtin_bit_cast(T, (uint32_t)w[1]));
+  }
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ int row_max(int v) { return over_row<LPR>(v, [](int a, int b) { return a > b ? a : b; }); }
+template <int LPR, typename T>
+__device__ __forceinline__ T row_sum(T v) { return over_row<LPR>(v, [](T a, T b) { return a + b; }); }
+
+// Integers in the order of the floats: negative ones with their magnitude turned over.  x + 0 makes -0 a 0.  What lies below NOT_LOWEST
+// is -inf (or a NaN with its sign bit); a NaN without it lies above all.
+constexpr int NOT_LOWEST = (int)0x80800000;
+__device__ __forceinline__ int turn(int u) { return u ^ ((u >> 31) & 0x7fffffff); }
+__device__ __forceinline__ int key_of(float x) { return turn(__float_as_int(x + 0.f)); }
+// the softmax's shift of a row whose largest key this is (a lower half that holds an index is none of the value's)
+template <typename T>
+__device__ __forceinline__ float top_of(int key) {
+  if (key < NOT_LOWEST) return 0.f;                          // (nothing but -inf)
+  return __int_as_float(sizeof(T) == 2 ? turn(key) & (int)0xffff0000 : turn(key));
 }
 
-template <int LPR>
-__device__ __forceinline__ float row_max(float v) {
+// y_j = e^(x_j - top) of a row (y may be x), and its sum.  As 2^(x_j L - top L), L = log2(e), in one fused step: the rounding of
+// top L is the whole row's and goes out with the sum, so a probability is off by |x_j - top| 2^-24 like that of a rounded
+// difference.  Where top L leaves float32 the difference is taken first.
+template <int LPR, int EPL>
+__device__ __forceinline__ float row_exp(float top, const float (&x)[EPL], float (&y)[EPL]) {
+  constexpr float L = 1.44269504f;
+  const float shift = top * L;
+  if (__any(fabsf(top) > 2e38f)) {
 #pragma unroll
-  for (int off = LPR / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
+    for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f((x[j] - top) * L);
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(x[j], L, -shift));
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) sum += y[j];
+  return row_sum<LPR>(sum);
 }
-template <int LPR>
-__device__ __forceinline__ float row_sum(float v) {
+
+// descending, by Batcher's odd-even merges
+template <int N>
+__device__ __forceinline__ void sort_descending(int (&s)[N]) {
 #pragma unroll
-  for (int off = LPR / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if ((i + j) / (2 * p) == (i + j + k) / (2 * p) && i + j + k < N) {
+            const int a = s[i + j], b = s[i + j + k];
+            s[i + j] = max(a, b);
+            s[i + j + k] = min(a, b);
+          }
+}
+
+// the k-th largest of a row (equal heads of several lanes count once); s: the lane's keys, sorted; top: the row's largest
+template <int LPR, int EPL>
+__device__ __forceinline__ int row_kth(int (&s)[EPL], int top, int top_k) {
+  int t = top;
+  if constexpr (LPR == 1) {
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) t = j < top_k ? +s[j] : t;
+  } else {
+    for (int k = 1; k < top_k; ++k) {
+      const bool mine = s[0] == t;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        const int here = s[j], next = j + 1 < EPL ? s[j + 1] : (int)0x80000000;
+        s[j] = mine ? +next : +here;
+      }
+      t = row_max<LPR>(s[0]);
+    }
+  }
+  return t;
 }
 
 // expert of element j of lane `sub` of a row: pieces of V consecutive experts, the lanes' pieces next to each other
@@ -96,8 +181,76 @@ __device__ __forceinline__ void load_row(const BalanceArgs& a, const T* row, int
   }
 }
 
+// cnt += the lane's chosen values of a row: those of at least the k-th largest key t
 template <typename T, int LPR, int EPL, int V>
-__global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs a) {
+__device__ __forceinline__ void choose(const int (&key)[EPL], int t, int sub, int top_k, int (&cnt)[EPL]) {
+  const int from = max(t, NOT_LOWEST);
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) cnt[j] += key[j] >= from;
+  } else {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) n += key[j] >= from;
+    if (__any(row_sum<LPR>(n) > top_k)) {                     // equal values: one by one, the largest that is left, the lowest index first
+      int s[EPL];
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) s[j] = key[j];
+      for (int k = 0; k < top_k; ++k) {
+        int best = s[0];
+#pragma unroll
+        for (int j = 1; j < EPL; ++j) best = max(best, s[j]);
+        best = row_max<LPR>(best);
+        int at = -BL_MAX_E;
+#pragma unroll
+        for (int j = EPL - 1; j >= 0; --j)
+          if (s[j] == best && best >= NOT_LOWEST) at = -expert_of<LPR, V>(j, sub);
+        at = -row_max<LPR>(at);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j)
+          if (expert_of<LPR, V>(j, sub) == at) { ++cnt[j]; s[j] = (int)0x80000000; }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) cnt[j] += key[j] >= from;
+    }
+  }
+}
+
+struct FinishArgs {
+  const float* psum;
+  const int* count;
+  const int* valid;
+  int groups, experts, top_k, blocks;
+  double coef;
+  double* term;              // [groups][column workgroups]: sum_e f P of the columns; behind them, [groups]: 1 where the group has rows
+  float* loss;
+  long* counts;              // [groups][experts]
+  float* prob;               // [groups][experts]
+  float* weight;             // [groups][experts] but for 1 / G', and, last, 1 / G'
+};
+
+// an expert's outputs, n: the group's rows; returns f P
+__device__ __forceinline__ double finish_expert(const FinishArgs& a, int g, int e, double p, long c, long n) {
+  const double some = n > 0 ? (double)n : 1.0, f = (double)c / (some * a.top_k), mean = p / some;
+  a.counts[(long)g * a.experts + e] = c;
+  a.prob[(long)g * a.experts + e] = (float)mean;
+  a.weight[(long)g * a.experts + e] = (float)(a.coef * a.experts * f / some);
+  return f * mean;
+}
+__device__ __forceinline__ void finish_loss(const FinishArgs& a, double sum, double some) {
+  const double share = some > 0 ? 1.0 / some : 0.0;
+  *a.loss = (float)(a.coef * a.experts * sum * share);
+  a.weight[(long)a.groups * a.experts] = (float)share;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+template <typename T, int LPR, int EPL, int V>
+__global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs a, FinishArgs f) {
   constexpr int RPW = 64 / LPR;                             // rows a wave works on at once
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPR, slot = lane / LPR;
   const int g = blockIdx.y;
@@ -108,47 +261,38 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
 #pragma unroll
   for (int j = 0; j < EPL; ++j) { psum[j] = 0.f; cnt[j] = 0; }
   const long step = (long)a.blocks * BL_WAVES * RPW;
-  for (long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW; n0 < a.rows; n0 += step) {
-    const long n = n0 + slot;
-    bool on = n < a.rows && (!mask || mask[n * a.mn]);
-    float x[EPL];
-    if (on) {
-      load_row<T, LPR, EPL, V>(a, x0 + n * a.sn, sub, x);
+  float next[EPL];
+  auto fetch = [&](long n) {                                // rows that do not count: -inf alone
+    if (n < a.rows && (!mask || mask[n * a.mn])) {
+      load_row<T, LPR, EPL, V>(a, x0 + n * a.sn, sub, next);
     } else {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) x[j] = -INFINITY;
+      for (int j = 0; j < EPL; ++j) next[j] = -INFINITY;
     }
-    float top = x[0];
+  };
+  long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW;
+  if (n0 < a.rows) fetch(n0 + slot);
+  for (; n0 < a.rows; n0 += step) {
+    float x[EPL];
+    int key[EPL], s[EPL];
 #pragma unroll
-    for (int j = 1; j < EPL; ++j) top = fmaxf(top, x[j]);
-    top = row_max<LPR>(top);
-    const float from = top == -INFINITY ? 0.f : top;
-    float y[EPL], sum = 0.f;
+    for (int j = 0; j < EPL; ++j) x[j] = next[j];
+    if (n0 + step < a.rows) fetch(n0 + step + slot);        // (under way while this row is worked on)
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) { y[j] = exp_neg(x[j] - from); sum += y[j]; }
-    sum = row_sum<LPR>(sum);
-    on = on && sum != 0.f;                                  // (all -inf: the row does not count; a NaN does)
-    const float inv = on ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) psum[j] += on ? y[j] * inv : 0.f;
-    valid += on && sub == 0;
-    // the choice, one expert a round: the largest value that is left, the lowest index where several have it
-    for (int k = 0; k < a.top_k; ++k) {
-      float best = -INFINITY;
-      int at = BL_MAX_E;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (x[j] > best) { best = x[j]; at = expert_of<LPR, V>(j, sub); }
-#pragma unroll
-      for (int off = LPR / 2; off > 0; off >>= 1) {
-        const float ob = __shfl_xor(best, off, 64);
-        const int oa = __shfl_xor(at, off, 64);
-        if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-      }
-#pragma unroll
-      for (int j = 0; j < EPL; ++j)
-        if (expert_of<LPR, V>(j, sub) == at) { ++cnt[j]; x[j] = -INFINITY; }
+    for (int j = 0; j < EPL; ++j) {
+      key[j] = key_of(x[j]);
+      if constexpr (sizeof(T) == 2) key[j] = (key[j] & (int)0xffff0000) | (0xffff - expert_of<LPR, V>(j, sub));
+      s[j] = key[j];
     }
+    sort_descending(s);
+    const int top = row_max<LPR>(s[0]);
+    const float sum = row_exp<LPR>(top_of<T>(top), x, x);
+    const bool counts = sum != 0.f;                         // (all -inf: the row does not count; a NaN does)
+    const float inv = counts ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) psum[j] = fmaf(x[j], inv, psum[j]);
+    valid += counts && sub == 0;
+    choose<T, LPR, EPL, V>(key, row_kth<LPR>(s, top, a.top_k), sub, a.top_k, cnt);
   }
   // the wave's rows, then the workgroup's waves
 #pragma unroll
@@ -163,6 +307,7 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
   for (int off = 32; off > 0; off >>= 1) valid += __shfl_xor(valid, off, 64);
   __shared__ float sp[BL_WAVES][LPR * EPL];
   __shared__ int sc[BL_WAVES][LPR * EPL], sv[BL_WAVES];
+  __shared__ double st[BL_WAVES];
   if (slot == 0) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
@@ -172,72 +317,74 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
   }
   if (lane == 0) sv[wave] = valid;
   __syncthreads();
+  int rows = 0;
+#pragma unroll
+  for (int w = 0; w < BL_WAVES; ++w) rows += sv[w];
+  const bool alone = gridDim.x == 1 && gridDim.y == 1;      // this workgroup has seen all rows: it finishes
   const long at = (long)g * a.blocks + blockIdx.x;
+  double term = 0;
   for (int e = threadIdx.x; e < a.experts; e += 64 * BL_WAVES) {
-    float p = 0.f;
+    double p = 0;
     int c = 0;
 #pragma unroll
     for (int w = 0; w < BL_WAVES; ++w) { p += sp[w][e]; c += sc[w][e]; }
-    a.psum[at * a.experts + e] = p;
-    a.count[at * a.experts + e] = c;
+    if (alone) {
+      term += finish_expert(f, 0, e, p, c, rows);
+    } else {
+      a.psum[at * a.experts + e] = (float)p;
+      a.count[at * a.experts + e] = c;
+    }
   }
+  if (!alone) {
+    if (threadIdx.x == 0) a.valid[at] = rows;
+    return;
+  }
+  term = wave_sum(term);
+  if (lane == 0) st[wave] = term;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    int v = 0;
-#pragma unroll
-    for (int w = 0; w < BL_WAVES; ++w) v += sv[w];
-    a.valid[at] = v;
+    term = 0;
+    for (int w = 0; w < BL_WAVES; ++w) term += st[w];
+    finish_loss(f, term, rows > 0 ? 1.0 : 0.0);
   }
 }
 
-struct FinishArgs {
-  const float* psum;
-  const int* count;
-  const int* valid;
-  int groups, experts, top_k, blocks;
-  double coef;
-  double* term;              // [groups][column workgroups]: sum_e f P of the columns
-  float* loss;
-  long* counts;              // [groups][experts]
-  float* prob;               // [groups][experts]
-  float* weight;             // [groups][experts] and, last, 1 / G'
-};
-
-// a group's 64 columns: counts, mean probabilities, weights (but for 1 / G') and this part of sum_e f_e P_e
+// BL_COLUMNS columns of a group: counts, mean probabilities, weights (but for 1 / G') and this part of sum_e f_e P_e
 __global__ __launch_bounds__(BL_FINISH) void balance_columns_kernel(FinishArgs a) {
-  const int g = blockIdx.y, col = threadIdx.x & 63, share = threadIdx.x >> 6, e = blockIdx.x * 64 + col;
-  constexpr int SHARES = BL_FINISH / 64;
-  __shared__ double sp[SHARES][64];
-  __shared__ long sc[SHARES][64], sn[BL_FINISH];
+  constexpr int SHARES = BL_FINISH / BL_COLUMNS, AHEAD = 8;
+  const int g = blockIdx.y, col = threadIdx.x % BL_COLUMNS, share = threadIdx.x / BL_COLUMNS, e = blockIdx.x * BL_COLUMNS + col;
+  __shared__ double sp[SHARES][BL_COLUMNS];
+  __shared__ long sc[SHARES][BL_COLUMNS], sn[BL_FINISH / 64];
   double p = 0;
   long c = 0, n = 0;
-  if (e < a.experts)
-    for (int b = share; b < a.blocks; b += SHARES) {
-      const long at = ((long)g * a.blocks + b) * a.experts + e;
-      p += a.psum[at];
-      c += a.count[at];
+  if (e < a.experts) {
+    const long at = (long)g * a.blocks * a.experts + e;
+    for (int b0 = share; b0 < a.blocks; b0 += AHEAD * SHARES) {
+      float v[AHEAD];
+      int w[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int b = b0 + u * SHARES;
+        v[u] = b < a.blocks ? a.psum[at + (long)b * a.experts] : 0.f;
+        w[u] = b < a.blocks ? a.count[at + (long)b * a.experts] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) { p += v[u]; c += w[u]; }
     }
+  }
   for (int b = threadIdx.x; b < a.blocks; b += BL_FINISH) n += a.valid[(long)g * a.blocks + b];
-  sp[share][col] = p;
-  sc[share][col] = c;
-  sn[threadIdx.x] = n;
-  __syncthreads();
-  if (share != 0) return;
-  p = 0; c = 0; n = 0;
-  for (int s = 0; s < SHARES; ++s) { p += sp[s][col]; c += sc[s][col]; }
-  for (int t = col; t < BL_FINISH; t += 64) n += sn[t];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-  double term = 0;
-  if (e < a.experts) {
-    const double some = n > 0 ? (double)n : 1.0, f = (double)c / (some * a.top_k), mean = p / some;
-    term = f * mean;
-    a.counts[(long)g * a.experts + e] = c;
-    a.prob[(long)g * a.experts + e] = (float)mean;
-    a.weight[(long)g * a.experts + e] = (float)(a.coef * a.experts * f / some);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) term += __shfl_xor(term, off, 64);
-  if (col == 0) {
+  sp[share][col] = p;
+  sc[share][col] = c;
+  if ((threadIdx.x & 63) == 0) sn[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  p = 0; c = 0; n = 0;
+  for (int s = 0; s < SHARES; ++s) { p += sp[s][col]; c += sc[s][col]; }
+  for (int w = 0; w < BL_FINISH / 64; ++w) n += sn[w];
+  const double term = wave_sum(share == 0 && e < a.experts ? finish_expert(a, g, e, p, c, n) : 0.0);
+  if (threadIdx.x == 0) {
     a.term[(long)g * gridDim.x + blockIdx.x] = term;
     if (blockIdx.x == 0) a.term[(long)a.groups * gridDim.x + g] = n > 0 ? 1.0 : 0.0;
   }
@@ -248,16 +395,14 @@ __global__ __launch_bounds__(BL_FINISH) void balance_loss_kernel(FinishArgs a, i
   for (long i = threadIdx.x; i < (long)a.groups * parts; i += BL_FINISH) sum += a.term[i];
   for (int g = threadIdx.x; g < a.groups; g += BL_FINISH) some += a.term[(long)a.groups * parts + g];
   __shared__ double ss[BL_FINISH / 64], sn[BL_FINISH / 64];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) { sum += __shfl_xor(sum, off, 64); some += __shfl_xor(some, off, 64); }
+  sum = wave_sum(sum);
+  some = wave_sum(some);
   if ((threadIdx.x & 63) == 0) { ss[threadIdx.x >> 6] = sum; sn[threadIdx.x >> 6] = some; }
   __syncthreads();
   if (threadIdx.x != 0) return;
   sum = some = 0;
   for (int w = 0; w < BL_FINISH / 64; ++w) { sum += ss[w]; some += sn[w]; }
-  const double share = some > 0 ? 1.0 / some : 0.0;
-  *a.loss = (float)(a.coef * a.experts * sum * share);
-  a.weight[(long)a.groups * a.experts] = (float)share;
+  finish_loss(a, sum, some);
 }
 
 template <typename T, int LPR, int EPL, int V>
@@ -286,16 +431,12 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs 
 #pragma unroll
       for (int j = 0; j < EPL; ++j) x[j] = -INFINITY;
     }
-    float top = x[0];
+    int top = key_of(x[0]);
 #pragma unroll
-    for (int j = 1; j < EPL; ++j) top = fmaxf(top, x[j]);
-    top = row_max<LPR>(top);
-    const float from = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, dot = 0.f;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) { x[j] = exp_neg(x[j] - from); sum += x[j]; }
-    sum = row_sum<LPR>(sum);
-    const float inv = on && sum != 0.f ? 1.f / sum : 0.f;
+    for (int j = 1; j < EPL; ++j) top = max(top, key_of(x[j]));
+    const float sum = row_exp<LPR>(top_of<float>(row_max<LPR>(top)), x, x);
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) { x[j] *= inv; dot += x[j] * w[j]; }
     dot = row_sum<LPR>(dot);
@@ -336,43 +477,50 @@ int lanes_per_row(int experts) {
   return lpr;
 }
 
-// workgroups per group: enough rows to fill them, and eight to a CU over all groups
-int blocks_for(long groups, long rows, int experts) {
+// workgroups per group: enough rows to fill them, two to a CU over all groups (they walk the rows that are left).  One group whose
+// rows a workgroup has done in four rounds stays with one: that saves the two launches that join partials.
+long rounds(long rows, int experts) {
   const long per = (long)BL_WAVES * (64 / lanes_per_row(experts));
-  const long want = (rows + per - 1) / per, most = groups >= 2048 ? 1 : 2048 / groups;
+  return (rows + per - 1) / per;
+}
+int walkers(long groups, long rows, int experts) {
+  const long want = rounds(rows, experts), most = groups >= BL_BLOCKS ? 1 : BL_BLOCKS / groups;
   return (int)(want < 1 ? 1 : want < most ? want : most);
+}
+int blocks_for(long groups, long rows, int experts) {
+  return groups == 1 && rounds(rows, experts) <= 4 ? 1 : walkers(groups, rows, experts);
 }
 
 template <typename T, bool BWD, int LPR, int EPL, int V>
-void launch_one(const BalanceArgs& a, hipStream_t s) {
+void launch_one(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   const dim3 grid((unsigned)a.blocks, (unsigned)a.groups), block(64 * BL_WAVES);
   if constexpr (BWD) hipLaunchKernelGGL((balance_bwd_kernel<T, LPR, EPL, V>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((balance_fwd_kernel<T, LPR, EPL, V>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((balance_fwd_kernel<T, LPR, EPL, V>), grid, block, 0, s, a, f);
 }
 
 template <typename T, bool BWD, int V>
-void launch(const BalanceArgs& a, hipStream_t s) {
+void launch(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   switch (lanes_per_row(a.experts)) {
-    case 1: return launch_one<T, BWD, 1, 8, V>(a, s);
-    case 2: return launch_one<T, BWD, 2, 8, V>(a, s);
-    case 4: return launch_one<T, BWD, 4, 8, V>(a, s);
-    case 8: return launch_one<T, BWD, 8, 8, V>(a, s);
-    case 16: return launch_one<T, BWD, 16, 8, V>(a, s);
-    case 32: return launch_one<T, BWD, 32, 8, V>(a, s);
-    default: return a.experts <= 512 ? launch_one<T, BWD, 64, 8, V>(a, s) : launch_one<T, BWD, 64, 16, V>(a, s);
+    case 1: return launch_one<T, BWD, 1, 8, V>(a, f, s);
+    case 2: return launch_one<T, BWD, 2, 8, V>(a, f, s);
+    case 4: return launch_one<T, BWD, 4, 8, V>(a, f, s);
+    case 8: return launch_one<T, BWD, 8, 8, V>(a, f, s);
+    case 16: return launch_one<T, BWD, 16, 8, V>(a, f, s);
+    case 32: return launch_one<T, BWD, 32, 8, V>(a, f, s);
+    default: return a.experts <= 512 ? launch_one<T, BWD, 64, 8, V>(a, f, s) : launch_one<T, BWD, 64, 16, V>(a, f, s);
   }
 }
 
 template <bool BWD>
-void dispatch(const BalanceArgs& a, int dtype, hipStream_t s) {
+void dispatch(const BalanceArgs& a, const FinishArgs& f, int dtype, hipStream_t s) {
   // 16-byte pieces where every row has them: consecutive experts, rows that start at 16 bytes and hold whole pieces
   const int per = dtype == REPMODE_F32 ? 4 : 8;
   auto whole = [&](const void* p, long sg, long sn, long se) {
     return ((uintptr_t)p & 15) == 0 && se == 1 && sn % per == 0 && (a.groups == 1 || sg % per == 0);
   };
   const bool vec = a.experts % per == 0 && whole(a.x, a.sg, a.sn, a.se) && (!BWD || whole(a.dx, a.dg, a.dn, a.de));
-  if (dtype == REPMODE_F32) vec ? launch<float, BWD, 4>(a, s) : launch<float, BWD, 1>(a, s);
-  else vec ? launch<bf16_t, BWD, 8>(a, s) : launch<bf16_t, BWD, 1>(a, s);
+  if (dtype == REPMODE_F32) vec ? launch<float, BWD, 4>(a, f, s) : launch<float, BWD, 1>(a, f, s);
+  else vec ? launch<bf16_t, BWD, 8>(a, f, s) : launch<bf16_t, BWD, 1>(a, f, s);
 }
 
 int check_shape(const char* who, const void* x, int dtype, long groups, long rows, int experts) {
@@ -389,7 +537,7 @@ extern "C" int repmode_balance_plan(long groups, long rows, int experts, long* w
   RM_REQUIRE(ws_bytes, "balance_plan: null pointer");
   if (int rc = check_shape("balance_plan", ws_bytes, REPMODE_F32, groups, rows, experts)) return rc;
   const long blocks = blocks_for(groups, rows, experts);
-  *ws_bytes = groups * ((experts + 63) / 64 + 1) * 8 + groups * blocks * experts * 8 + groups * blocks * 4;
+  *ws_bytes = groups * ((experts + BL_COLUMNS - 1) / BL_COLUMNS + 1) * 8 + groups * blocks * experts * 8 + groups * blocks * 4;
   return REPMODE_OK;
 }
 
@@ -403,7 +551,7 @@ extern "C" int repmode_balance_fwd(const void* x, int dtype, long groups, long r
   long need = 0;
   if (int rc = repmode_balance_plan(groups, rows, experts, &need)) return rc;
   RM_REQUIRE(ws_bytes >= need && ((uintptr_t)ws & 7) == 0, "balance_fwd: workspace of %ld bytes (8-byte aligned) needed, got %ld", need, ws_bytes);
-  const int parts = (experts + 63) / 64;
+  const int parts = (experts + BL_COLUMNS - 1) / BL_COLUMNS;
   BalanceArgs a{};
   a.x = x; a.mask = mask;
   a.sg = sg; a.sn = sn; a.se = se; a.mg = mg; a.mn = mn;
@@ -414,9 +562,10 @@ extern "C" int repmode_balance_fwd(const void* x, int dtype, long groups, long r
   a.count = reinterpret_cast<int*>(a.psum + groups * a.blocks * experts);
   a.valid = a.count + groups * a.blocks * experts;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  dispatch<false>(a, dtype, s);
+  const FinishArgs f{a.psum, a.count, a.valid, a.groups, experts, top_k, a.blocks, coef, term, loss, counts, prob, weight};
+  dispatch<false>(a, f, dtype, s);
   RM_LAUNCH_CHECK("balance_fwd");
-  FinishArgs f{a.psum, a.count, a.valid, a.groups, experts, top_k, a.blocks, coef, term, loss, counts, prob, weight};
+  if (groups == 1 && a.blocks == 1) return REPMODE_OK;
   hipLaunchKernelGGL(balance_columns_kernel, dim3(parts, (unsigned)groups), dim3(BL_FINISH), 0, s, f);
   RM_LAUNCH_CHECK("balance_columns");
   hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(BL_FINISH), 0, s, f, parts);
@@ -434,8 +583,8 @@ extern "C" int repmode_balance_bwd(const void* x, int dtype, long groups, long r
   a.x = x; a.mask = mask; a.dx = dx; a.weight = weight; a.up = up;
   a.sg = sg; a.sn = sn; a.se = se; a.mg = mg; a.mn = mn; a.dg = dg; a.dn = dn; a.de = de;
   a.rows = rows; a.groups = (int)groups; a.experts = experts;
-  a.blocks = blocks_for(groups, rows, experts);
-  dispatch<true>(a, dtype, static_cast<hipStream_t>(stream));
+  a.blocks = walkers(groups, rows, experts);
+  dispatch<true>(a, FinishArgs{}, dtype, static_cast<hipStream_t>(stream));
   RM_LAUNCH_CHECK("balance_bwd");
   return REPMODE_OK;
 }

@@ -37,7 +37,8 @@ def _balance_ref(x, top_k, mask, coef, up=1.0):
     w = up * scale * f / some
     dot = (p * w[:, None]).sum(2, keepdim=True)
     grad = p * (w[:, None] - dot)
-    # a probability: x - max rounds once (its distance to the maximum, D, times U), exp within 4 U, at most 20 sums, reciprocal and product
+    # a probability: the rounding of its distance D to the maximum (times log2(e), in one step with it: D U and, of log2(e) itself,
+    # 0.23 D U, taken from the 28 U for D < 20; above, the probability is below 2e-9), exp within 4 U, at most 20 sums, reciprocal, product
     far = torch.where(p > 0, x.amax(2, keepdim=True) - x, torch.zeros(())).clamp(max=110)
     rel = (far + 28) * U
     off = (p * rel).sum(2, keepdim=True) + rel                       # (the sum's own error, weighted by what it sums)
