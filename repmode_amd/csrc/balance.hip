@@ -21,14 +21,16 @@
 // What bounds it: HBM for the backward pass (one read, one write), the instructions of exponential and choice for forward passes.
 #include "common.h"
 
+#include <atomic>
 #include <cmath>
 
 namespace {
 
 constexpr int BL_WAVES = 8;
 constexpr int BL_MAX_E = REPMODE_BALANCE_MAX_EXPERTS;
+constexpr int BL_TILE_BYTES = 72 << 10;  // of a tile: two workgroups share a CU's LDS
 constexpr int BL_FINISH = 256;           // threads of the finish
-constexpr int BL_COLUMNS = 8;            // columns of a workgroup of it; the other threads share the partials
+constexpr int BL_COLUMNS = 4;            // columns of a workgroup of it; the other threads share the partials
 constexpr int BL_BLOCKS = 512;           // most workgroups of a pass: two to a CU, which registers leave room for
 
 struct BalanceArgs {
@@ -43,6 +45,7 @@ struct BalanceArgs {
   long rows;
   int groups, experts, top_k;
   int blocks;                // workgroups per group
+  int tile_rows, pitch;      // tiled: rows of a tile, floats from one of them to the next in LDS
   float* psum;               // forward: [groups][blocks][experts]
   int* count;                //          the same shape
   int* valid;                //          [groups][blocks]
@@ -125,6 +128,28 @@ __device__ __forceinline__ void sort_descending(int (&s)[N]) {
           }
 }
 
+// the lane whose head is t moves its list up by one, as far as N values of it are looked at afterwards
+template <int N, int EPL>
+__device__ __forceinline__ void pop(int (&s)[EPL], int t) {
+  const bool mine = s[0] == t;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int here = s[j], next = j + 1 < EPL ? s[j + 1] : (int)0x80000000;
+    s[j] = mine ? +next : +here;
+  }
+}
+// rounds K + 1 .. top_k of at most EPL: after the K-th, EPL - K values of a list can still count
+template <int LPR, int K, int EPL>
+__device__ __forceinline__ int rounds_from(int (&s)[EPL], int t, int top_k) {
+  if constexpr (K < EPL) {
+    if (K < top_k) {
+      pop<EPL - K>(s, t);
+      return rounds_from<LPR, K + 1>(s, row_max<LPR>(s[0]), top_k);
+    }
+  }
+  return t;
+}
+
 // the k-th largest of a row (equal heads of several lanes count once); s: the lane's keys, sorted; top: the row's largest
 template <int LPR, int EPL>
 __device__ __forceinline__ int row_kth(int (&s)[EPL], int top, int top_k) {
@@ -132,14 +157,11 @@ __device__ __forceinline__ int row_kth(int (&s)[EPL], int top, int top_k) {
   if constexpr (LPR == 1) {
 #pragma unroll
     for (int j = 1; j < EPL; ++j) t = j < top_k ? +s[j] : t;
+  } else if (top_k <= EPL) {
+    t = rounds_from<LPR, 1>(s, t, top_k);
   } else {
     for (int k = 1; k < top_k; ++k) {
-      const bool mine = s[0] == t;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) {
-        const int here = s[j], next = j + 1 < EPL ? s[j + 1] : (int)0x80000000;
-        s[j] = mine ? +next : +here;
-      }
+      pop<EPL>(s, t);
       t = row_max<LPR>(s[0]);
     }
   }
@@ -150,34 +172,56 @@ __device__ __forceinline__ int row_kth(int (&s)[EPL], int top, int top_k) {
 template <int LPR, int V>
 __device__ __forceinline__ int expert_of(int j, int sub) { return (j / V) * (LPR * V) + sub * V + j % V; }
 
+// a lane's values of a row; -inf where there is none, and everywhere in a row that does not count
 template <typename T, int LPR, int EPL, int V>
-__device__ __forceinline__ void load_row(const BalanceArgs& a, const T* row, int sub, float (&x)[EPL]) {
-  if constexpr (V > 1) {
+__device__ __forceinline__ void load_row(const BalanceArgs& a, const T* row, bool on, int sub, float (&x)[EPL]) {
 #pragma unroll
-    for (int j = 0; j < EPL; j += V) {
-      const int e = expert_of<LPR, V>(j, sub);
-      if (e < a.experts) {                                  // (V divides the experts here)
-        const u32x4 w = *reinterpret_cast<const u32x4*>(row + e);
+  for (int j = 0; j < EPL; ++j) x[j] = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (sizeof(T) == 4) {
-            x[j + k] = __uint_as_float(w[k]);
-          } else {
-            x[j + 2 * k] = __uint_as_float(w[k] << 16);
-            x[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-          }
+  for (int j = 0; j < EPL; j += V) {
+    const int e = expert_of<LPR, V>(j, sub);
+    if (!on || e >= a.experts) continue;                    // (V divides the experts)
+    if constexpr (V == 1) {
+      x[j] = to_f32<T>(row[(long)e * a.se]);
+    } else {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(row + e);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          x[j + k] = __uint_as_float(w[k]);
+        } else {
+          x[j + 2 * k] = __uint_as_float(w[k] << 16);
+          x[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) x[j + k] = -INFINITY;
       }
     }
-  } else {
+  }
+}
+
+// Logits whose rows, not experts, are neighbours in memory: a tile of rows is read along them into LDS, [row][expert] with an odd
+// pitch, and the rows taken from there.  (Read directly a wave would use 4 RPW bytes of each cache line it asks for.)
+template <typename T>
+__device__ __forceinline__ void load_tile(const BalanceArgs& a, const T* x0, const uint8_t* mask, long n0, float* tile) {
+  constexpr int AHEAD = 8;
+  const int r = threadIdx.x % a.tile_rows, e0 = threadIdx.x / a.tile_rows, step = 64 * BL_WAVES / a.tile_rows;
+  const long n = n0 + r;
+  const bool on = n < a.rows && (!mask || mask[n * a.mn]);
+  const T* x = x0 + n * a.sn;
+  for (int e = e0; e < a.experts; e += AHEAD * step) {
+    float v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      const int e = expert_of<LPR, 1>(j, sub);
-      x[j] = e < a.experts ? to_f32<T>(row[(long)e * a.se]) : -INFINITY;
-    }
+    for (int u = 0; u < AHEAD; ++u) v[u] = on && e + u * step < a.experts ? to_f32<T>(x[(long)(e + u * step) * a.se]) : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (e + u * step < a.experts) tile[r * a.pitch + e + u * step] = v[u];
+  }
+}
+template <int LPR, int EPL>
+__device__ __forceinline__ void row_of_tile(const BalanceArgs& a, const float* tile, int r, int sub, float (&x)[EPL]) {
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) {
+    const int e = expert_of<LPR, 1>(j, sub);
+    x[j] = e < a.experts ? tile[r * a.pitch + e] : -INFINITY;
   }
 }
 
@@ -189,9 +233,10 @@ __device__ __forceinline__ void choose(const int (&key)[EPL], int t, int sub, in
 #pragma unroll
     for (int j = 0; j < EPL; ++j) cnt[j] += key[j] >= from;
   } else {
+    bool in[EPL];
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) n += key[j] >= from;
+    for (int j = 0; j < EPL; ++j) { in[j] = key[j] >= from; n += in[j]; }
     if (__any(row_sum<LPR>(n) > top_k)) {                     // equal values: one by one, the largest that is left, the lowest index first
       int s[EPL];
 #pragma unroll
@@ -212,7 +257,7 @@ __device__ __forceinline__ void choose(const int (&key)[EPL], int t, int sub, in
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) cnt[j] += key[j] >= from;
+      for (int j = 0; j < EPL; ++j) cnt[j] += in[j];
     }
   }
 }
@@ -249,10 +294,10 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-template <typename T, int LPR, int EPL, int V>
+template <typename T, int LPR, int EPL, int V, bool TILED>
 __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs a, FinishArgs f) {
   constexpr int RPW = 64 / LPR;                             // rows a wave works on at once
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPR, slot = lane / LPR;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % LPR, slot = lane / LPR;
   const int g = blockIdx.y;
   const T* x0 = static_cast<const T*>(a.x) + (long)g * a.sg;
   const uint8_t* mask = a.mask ? a.mask + (long)g * a.mg : nullptr;
@@ -260,24 +305,8 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
   int cnt[EPL], valid = 0;
 #pragma unroll
   for (int j = 0; j < EPL; ++j) { psum[j] = 0.f; cnt[j] = 0; }
-  const long step = (long)a.blocks * BL_WAVES * RPW;
-  float next[EPL];
-  auto fetch = [&](long n) {                                // rows that do not count: -inf alone
-    if (n < a.rows && (!mask || mask[n * a.mn])) {
-      load_row<T, LPR, EPL, V>(a, x0 + n * a.sn, sub, next);
-    } else {
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) next[j] = -INFINITY;
-    }
-  };
-  long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW;
-  if (n0 < a.rows) fetch(n0 + slot);
-  for (; n0 < a.rows; n0 += step) {
-    float x[EPL];
+  auto work = [&](float (&x)[EPL]) {
     int key[EPL], s[EPL];
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) x[j] = next[j];
-    if (n0 + step < a.rows) fetch(n0 + step + slot);        // (under way while this row is worked on)
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       key[j] = key_of(x[j]);
@@ -288,11 +317,43 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
     const int top = row_max<LPR>(s[0]);
     const float sum = row_exp<LPR>(top_of<T>(top), x, x);
     const bool counts = sum != 0.f;                         // (all -inf: the row does not count; a NaN does)
-    const float inv = counts ? 1.f / sum : 0.f;
+    const float inv = counts ? __builtin_amdgcn_rcpf(sum) : 0.f;         // (1 ulp; 1 <= sum <= experts)
 #pragma unroll
     for (int j = 0; j < EPL; ++j) psum[j] = fmaf(x[j], inv, psum[j]);
     valid += counts && sub == 0;
     choose<T, LPR, EPL, V>(key, row_kth<LPR>(s, top, a.top_k), sub, a.top_k, cnt);
+  };
+  if constexpr (TILED) {
+    extern __shared__ float tile[];
+    for (long n0 = (long)blockIdx.x * a.tile_rows; n0 < a.rows; n0 += (long)a.blocks * a.tile_rows) {
+      load_tile(a, x0, mask, n0, tile);
+      __syncthreads();
+      for (int r = wave * RPW; r < a.tile_rows; r += BL_WAVES * RPW) {
+        float x[EPL];
+        row_of_tile<LPR>(a, tile, r + slot, sub, x);
+        work(x);
+      }
+      __syncthreads();
+    }
+  } else {
+    const long step = (long)a.blocks * BL_WAVES * RPW;
+    float next[EPL];
+    long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW;
+    const T* row = x0 + (n0 + slot) * a.sn;
+    long masked = (n0 + slot) * a.mn;
+    auto fetch = [&](long n) {
+      load_row<T, LPR, EPL, V>(a, row, n < a.rows && (!mask || mask[masked]), sub, next);
+      row += step * a.sn;
+      masked += step * a.mn;
+    };
+    if (n0 < a.rows) fetch(n0 + slot);
+    for (; n0 < a.rows; n0 += step) {
+      float x[EPL];
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) x[j] = next[j];
+      if (n0 + step < a.rows) fetch(n0 + step + slot);      // (under way while this row is worked on)
+      work(x);
+    }
   }
   // the wave's rows, then the workgroup's waves
 #pragma unroll
@@ -405,10 +466,10 @@ __global__ __launch_bounds__(BL_FINISH) void balance_loss_kernel(FinishArgs a, i
   finish_loss(a, sum, some);
 }
 
-template <typename T, int LPR, int EPL, int V>
+template <typename T, int LPR, int EPL, int V, bool TILED>
 __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs a) {
   constexpr int RPW = 64 / LPR;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPR, slot = lane / LPR;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane % LPR, slot = lane / LPR;
   const int g = blockIdx.y;
   const T* x0 = static_cast<const T*>(a.x) + (long)g * a.sg;
   T* d0 = static_cast<T*>(a.dx) + (long)g * a.dg;
@@ -420,28 +481,54 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs 
     const int e = expert_of<LPR, V>(j, sub);
     w[j] = e < a.experts ? scale * a.weight[(long)g * a.experts + e] : 0.f;
   }
-  const long step = (long)a.blocks * BL_WAVES * RPW;
-  for (long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW; n0 < a.rows; n0 += step) {
-    const long n = n0 + slot;
-    const bool in = n < a.rows, on = in && (!mask || mask[n * a.mn]);
-    float x[EPL];
-    if (on) {
-      load_row<T, LPR, EPL, V>(a, x0 + n * a.sn, sub, x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) x[j] = -INFINITY;
-    }
+  auto work = [&](float (&x)[EPL]) {                        // logits in, gradients out
     int top = key_of(x[0]);
 #pragma unroll
     for (int j = 1; j < EPL; ++j) top = max(top, key_of(x[j]));
     const float sum = row_exp<LPR>(top_of<float>(row_max<LPR>(top)), x, x);
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    const float inv = sum != 0.f ? __builtin_amdgcn_rcpf(sum) : 0.f;
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) { x[j] *= inv; dot += x[j] * w[j]; }
     dot = row_sum<LPR>(dot);
 #pragma unroll
     for (int j = 0; j < EPL; ++j) x[j] = sum != 0.f ? x[j] * (w[j] - dot) : 0.f;      // (a row that does not count: 0 whatever w is)
+  };
+  if constexpr (TILED) {
+    extern __shared__ float tile[];
+    const int r = threadIdx.x % a.tile_rows, e0 = threadIdx.x / a.tile_rows, estep = 64 * BL_WAVES / a.tile_rows;
+    for (long n0 = (long)blockIdx.x * a.tile_rows; n0 < a.rows; n0 += (long)a.blocks * a.tile_rows) {
+      load_tile(a, x0, mask, n0, tile);
+      __syncthreads();
+      for (int q = wave * RPW; q < a.tile_rows; q += BL_WAVES * RPW) {
+        float x[EPL];
+        row_of_tile<LPR>(a, tile, q + slot, sub, x);
+        work(x);
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          const int e = expert_of<LPR, 1>(j, sub);
+          if (e < a.experts) tile[(q + slot) * a.pitch + e] = x[j];
+        }
+      }
+      __syncthreads();
+      if (n0 + r < a.rows) {
+        T* d = d0 + (n0 + r) * a.dn;
+        for (int e = e0; e < a.experts; e += estep) {
+          if constexpr (sizeof(T) == 4) d[(long)e * a.de] = tile[r * a.pitch + e];
+          else d[(long)e * a.de] = f32_to_bf16(tile[r * a.pitch + e]);
+        }
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  const long step = (long)a.blocks * BL_WAVES * RPW;
+  for (long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW; n0 < a.rows; n0 += step) {
+    const long n = n0 + slot;
+    const bool in = n < a.rows, on = in && (!mask || mask[n * a.mn]);
+    float x[EPL];
+    load_row<T, LPR, EPL, V>(a, x0 + n * a.sn, on, sub, x);
+    work(x);
     if (!in) continue;
     T* row = d0 + n * a.dn;
     if constexpr (V > 1) {
@@ -491,36 +578,73 @@ int blocks_for(long groups, long rows, int experts) {
   return groups == 1 && rounds(rows, experts) <= 4 ? 1 : walkers(groups, rows, experts);
 }
 
-template <typename T, bool BWD, int LPR, int EPL, int V>
-void launch_one(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
+template <typename T, bool BWD, int LPR, int EPL, int V, bool TILED>
+int launch_one(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   const dim3 grid((unsigned)a.blocks, (unsigned)a.groups), block(64 * BL_WAVES);
-  if constexpr (BWD) hipLaunchKernelGGL((balance_bwd_kernel<T, LPR, EPL, V>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((balance_fwd_kernel<T, LPR, EPL, V>), grid, block, 0, s, a, f);
+  const size_t lds = TILED ? (size_t)a.tile_rows * a.pitch * sizeof(float) : 0;
+  if constexpr (TILED) {
+    static std::atomic<unsigned> allowed{0};                // per device: the tile may take more than 64 KiB
+    int dev = 0;
+    RM_HIP(hipGetDevice(&dev));
+    if (!(allowed.load() >> (dev & 31) & 1)) {
+      const void* kernel;
+      if constexpr (BWD) kernel = reinterpret_cast<const void*>(&balance_bwd_kernel<T, LPR, EPL, V, TILED>);
+      else kernel = reinterpret_cast<const void*>(&balance_fwd_kernel<T, LPR, EPL, V, TILED>);
+      RM_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, BL_TILE_BYTES));
+      allowed.fetch_or(1u << (dev & 31));
+    }
+  }
+  if constexpr (BWD) hipLaunchKernelGGL((balance_bwd_kernel<T, LPR, EPL, V, TILED>), grid, block, lds, s, a);
+  else hipLaunchKernelGGL((balance_fwd_kernel<T, LPR, EPL, V, TILED>), grid, block, lds, s, a, f);
+  RM_LAUNCH_CHECK(BWD ? "balance_bwd" : "balance_fwd");
+  return REPMODE_OK;
 }
 
-template <typename T, bool BWD, int V>
-void launch(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
+template <typename T, bool BWD, int V, bool TILED>
+int launch(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   switch (lanes_per_row(a.experts)) {
-    case 1: return launch_one<T, BWD, 1, 8, V>(a, f, s);
-    case 2: return launch_one<T, BWD, 2, 8, V>(a, f, s);
-    case 4: return launch_one<T, BWD, 4, 8, V>(a, f, s);
-    case 8: return launch_one<T, BWD, 8, 8, V>(a, f, s);
-    case 16: return launch_one<T, BWD, 16, 8, V>(a, f, s);
-    case 32: return launch_one<T, BWD, 32, 8, V>(a, f, s);
-    default: return a.experts <= 512 ? launch_one<T, BWD, 64, 8, V>(a, f, s) : launch_one<T, BWD, 64, 16, V>(a, f, s);
+    case 1: return launch_one<T, BWD, 1, 8, V, false>(a, f, s);
+    case 2: return launch_one<T, BWD, 2, 8, V, false>(a, f, s);
+    case 4: return launch_one<T, BWD, 4, 8, V, false>(a, f, s);
+    case 8: return launch_one<T, BWD, 8, 8, V, TILED>(a, f, s);
+    case 16: return launch_one<T, BWD, 16, 8, V, TILED>(a, f, s);
+    case 32: return launch_one<T, BWD, 32, 8, V, TILED>(a, f, s);
+    default: return a.experts <= 512 ? launch_one<T, BWD, 64, 8, V, TILED>(a, f, s) : launch_one<T, BWD, 64, 16, V, TILED>(a, f, s);
   }
 }
 
+// A pass with the form its strides ask for:
+//   16-byte pieces where every row has them: consecutive experts, rows that start at 16 bytes and hold whole pieces;
+//   tiles where the rows are neighbours and a row takes 8 lanes or more, so that a wave's loads along the experts would take 32 bytes
+// or less of a cache line (2^26 float32 logits, 32 / 64 / 128 / 512 experts, tiles and without: forward 103 / 104 / 101 / 145 us and
+// 76 / 103 / 194 / 556, backward 166 / 157 / 152 / 163 and 198 / 278 / 473 / 1056; bfloat16 backward 165 / 179 / 176 / 187 and 132 /
+// 190 / 295 / 1485).  Not for the forward pass of bfloat16, whose tiles' 2-byte loads cost what they save (149 / 147 / 260 and 123 /
+// 143 / 230);
+//   else element by element.
 template <bool BWD>
-void dispatch(const BalanceArgs& a, const FinishArgs& f, int dtype, hipStream_t s) {
-  // 16-byte pieces where every row has them: consecutive experts, rows that start at 16 bytes and hold whole pieces
+int dispatch(BalanceArgs a, FinishArgs* finish, int dtype, hipStream_t s) {
+  FinishArgs f{};
+  if (finish) f = *finish;
   const int per = dtype == REPMODE_F32 ? 4 : 8;
   auto whole = [&](const void* p, long sg, long sn, long se) {
     return ((uintptr_t)p & 15) == 0 && se == 1 && sn % per == 0 && (a.groups == 1 || sg % per == 0);
   };
-  const bool vec = a.experts % per == 0 && whole(a.x, a.sg, a.sn, a.se) && (!BWD || whole(a.dx, a.dg, a.dn, a.de));
-  if (dtype == REPMODE_F32) vec ? launch<float, BWD, 4>(a, f, s) : launch<float, BWD, 1>(a, f, s);
-  else vec ? launch<bf16_t, BWD, 8>(a, f, s) : launch<bf16_t, BWD, 1>(a, f, s);
+  if (a.experts % per == 0 && whole(a.x, a.sg, a.sn, a.se) && (!BWD || whole(a.dx, a.dg, a.dn, a.de)))
+    return dtype == REPMODE_F32 ? launch<float, BWD, 4, false>(a, f, s) : launch<bf16_t, BWD, 8, false>(a, f, s);
+  if (a.se != 1 && a.sn == 1 && lanes_per_row(a.experts) >= 8 && (BWD || dtype == REPMODE_F32)) {
+    a.pitch = a.experts | 1;
+    a.tile_rows = 64 * BL_WAVES;
+    while ((size_t)a.tile_rows * a.pitch * sizeof(float) > BL_TILE_BYTES) a.tile_rows /= 2;
+    const long tiles = (a.rows + a.tile_rows - 1) / a.tile_rows;
+    // (a tile is rows for at least two rounds of the workgroup, so there are never more workgroups than the plan has)
+    if (tiles < a.blocks) a.blocks = (int)(tiles < 1 ? 1 : tiles);
+    if (finish) finish->blocks = f.blocks = a.blocks;
+    if constexpr (BWD) {
+      if (dtype == REPMODE_BF16) return launch<bf16_t, BWD, 1, true>(a, f, s);
+    }
+    return launch<float, BWD, 1, true>(a, f, s);
+  }
+  return dtype == REPMODE_F32 ? launch<float, BWD, 1, false>(a, f, s) : launch<bf16_t, BWD, 1, false>(a, f, s);
 }
 
 int check_shape(const char* who, const void* x, int dtype, long groups, long rows, int experts) {
@@ -562,10 +686,9 @@ extern "C" int repmode_balance_fwd(const void* x, int dtype, long groups, long r
   a.count = reinterpret_cast<int*>(a.psum + groups * a.blocks * experts);
   a.valid = a.count + groups * a.blocks * experts;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const FinishArgs f{a.psum, a.count, a.valid, a.groups, experts, top_k, a.blocks, coef, term, loss, counts, prob, weight};
-  dispatch<false>(a, f, dtype, s);
-  RM_LAUNCH_CHECK("balance_fwd");
-  if (groups == 1 && a.blocks == 1) return REPMODE_OK;
+  FinishArgs f{a.psum, a.count, a.valid, a.groups, experts, top_k, a.blocks, coef, term, loss, counts, prob, weight};
+  if (int rc = dispatch<false>(a, &f, dtype, s)) return rc;
+  if (groups == 1 && f.blocks == 1) return REPMODE_OK;
   hipLaunchKernelGGL(balance_columns_kernel, dim3(parts, (unsigned)groups), dim3(BL_FINISH), 0, s, f);
   RM_LAUNCH_CHECK("balance_columns");
   hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(BL_FINISH), 0, s, f, parts);
@@ -584,7 +707,5 @@ extern "C" int repmode_balance_bwd(const void* x, int dtype, long groups, long r
   a.sg = sg; a.sn = sn; a.se = se; a.mg = mg; a.mn = mn; a.dg = dg; a.dn = dn; a.de = de;
   a.rows = rows; a.groups = (int)groups; a.experts = experts;
   a.blocks = walkers(groups, rows, experts);
-  dispatch<true>(a, FinishArgs{}, dtype, static_cast<hipStream_t>(stream));
-  RM_LAUNCH_CHECK("balance_bwd");
-  return REPMODE_OK;
+  return dispatch<true>(a, nullptr, dtype, static_cast<hipStream_t>(stream));
 }

@@ -101,6 +101,20 @@ def test_balance_loss_strides(dtype):
     _check_balance(base[:, ::2, :64], 3, (torch.rand(6, 48, generator=gen) < 0.5).to(DEV)[:, ::2])
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('groups, rows, experts, top_k', [
+    (None, 1, 9, 2), (None, 513, 16, 2), (None, 1100, 17, 3), (2, 300, 33, 4), (None, 257, 64, 6), (3, 129, 100, 2), (None, 130, 256, 8),
+    (None, 33, 300, 1), (2, 70, 512, 9), (None, 17, 513, 2), (None, 40, 1024, 16), (None, 20000, 24, 2)])
+def test_balance_loss_rows_adjacent(groups, rows, experts, top_k, dtype):
+    """Logits whose rows are neighbours in memory, experts the slow axis; with a mask, and rows that a tile's end cuts."""
+    gen = torch.Generator().manual_seed(rows + experts)
+    shape = (experts, rows) if groups is None else (groups, experts, rows)
+    x = (torch.randn(shape, generator=gen) * 2).to(DEV, dtype).transpose(-2, -1)
+    _check_balance(x, top_k)
+    mask = (torch.rand(x.shape[:-1], generator=gen) < 0.6).to(DEV)
+    _check_balance(torch.where(mask[..., None], x, math.nan).transpose(-2, -1).contiguous().transpose(-2, -1), top_k, mask)
+
+
 @pytest.mark.parametrize('experts', [4, 8, 40, 256, 640])
 def test_balance_loss_ties_and_infinities(experts):
     """Equal logits go to the lowest index; -inf is never chosen, even where fewer than top_k experts are left; a row of -inf alone
