@@ -183,6 +183,17 @@ def load_torch_ops():
     install_foreign_step_hook()
 
 
+def load_list_ops():
+    """The operator library as a Python module (``grad_norm``, ``adamw_step``; the end of csrc/torch/repmode_ops.cpp)."""
+    import importlib.machinery
+    import importlib.util
+    load_torch_ops()
+    loader = importlib.machinery.ExtensionFileLoader('librepmode_torch', TORCH_LIB_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader('librepmode_torch', loader))
+    loader.exec_module(module)
+    return module
+
+
 def torch_ops_loaded():
     return _torch_ops_loaded
 

@@ -32,9 +32,9 @@ if [ "${REPMODE_SKIP_TORCH_OPS:-0}" != "1" ]; then
     TDIR="$(python3 -c 'import os, torch; print(os.path.dirname(torch.__file__))')"
     ABI="$(python3 -c 'import torch; print(int(torch._C._GLIBCXX_USE_CXX11_ABI))')"
     g++ -O2 -std=c++17 -fPIC -shared -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -D_GLIBCXX_USE_CXX11_ABI=$ABI \
-        -I"$TDIR/include" -I"$TDIR/include/torch/csrc/api/include" -I/opt/rocm/include -I"$ROOT/include" \
+        -I"$(python3 -c 'import sysconfig; print(sysconfig.get_paths()["include"])')" -I"$TDIR/include" -I"$TDIR/include/torch/csrc/api/include" -I/opt/rocm/include -I"$ROOT/include" \
         "$TSRC" -o "$TOUT" \
-        -L"$TDIR/lib" -ltorch -ltorch_cpu -lc10 -lc10_hip -ltorch_hip \
+        -L"$TDIR/lib" -ltorch_python -ltorch -ltorch_cpu -lc10 -lc10_hip -ltorch_hip \
         -L"$(dirname "$OUT")" -l:"$(basename "$OUT")" -L/opt/rocm/lib -lamdhip64 -Wl,-rpath,'$ORIGIN'
   fi
   echo "built $TOUT"

@@ -12,10 +12,14 @@
 // autograd bookkeeping -- the counterpart of what fnet/nn_modules/RepMode.py:171-214 leaves to stock PyTorch ops.
 //
 // Built by repmode_amd/csrc/build.sh into repmode_amd/librepmode_torch.so (in-tree, next to librepmode_hip.so).
+#include <torch/csrc/python_headers.h>
+
 #include <ATen/ATen.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/autograd.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -1821,33 +1825,46 @@ void op_adam_step_dev(const std::vector<Tensor>& params, const std::vector<Tenso
 // The norm of many tensors and AdamW over many tensors (csrc/grad_norm.hip, csrc/adamw.hip).
 // A tensor is flat here: its elements in memory order, so it has to be dense, and a gradient of other strides than its
 // parameter's is brought into the parameter's order first.
-std::tuple<Tensor, Tensor> op_grad_norm(const std::vector<Tensor>& tensors, double max_norm) {
+// These two take lists of hundreds of tensors, which the dispatcher boxes one by one (0.1 us each: 80 us for the four lists of 193
+// parameters, more than their kernels take).  Python reaches them as functions of this library's own module (the end of this file), as
+// torch's own functions over lists are reached; a list is the addresses of the tensors that its Python objects hold.
+struct TensorList {
+  std::vector<const Tensor*> t;
+  size_t size() const { return t.size(); }
+  bool empty() const { return t.empty(); }
+  const Tensor& get(size_t i) const { return *t[i]; }
+};
+
+std::tuple<Tensor, Tensor> op_grad_norm(const TensorList& tensors, double max_norm) {
   TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
   TORCH_CHECK(max_norm >= 0, "grad_norm: max_norm must not be negative or NaN, got ", max_norm);
-  for (size_t i = 0; i < tensors.size(); ++i) {
-    const Tensor& t = tensors[i];
+  const size_t n = tensors.size();
+  const at::Device dev = tensors.get(0).device();
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& t = tensors.get(i);
     require_hip(t, "grad_norm: tensor");
     (void)dtype_code(t.scalar_type());
-    TORCH_CHECK(t.device() == tensors[0].device(), "grad_norm: tensor ", i, " is on ", t.device(), ", tensor 0 on ", tensors[0].device());
+    TORCH_CHECK(t.device() == dev, "grad_norm: tensor ", i, " is on ", t.device(), ", tensor 0 on ", dev);
   }
-  DeviceGuard guard(tensors[0].device());
+  DeviceGuard guard(dev);
   at::NoGradGuard no_grad;
   std::vector<const void*> x[2];
   std::vector<long> numel[2];
   std::vector<Tensor> hold;
   long room = 0;
-  for (const Tensor& t0 : tensors) {
-    if (t0.numel() == 0) continue;
-    Tensor t = t0;
-    if (!t.is_non_overlapping_and_dense()) hold.push_back(t = t0.contiguous());        // (any order of the elements has the same norm)
+  for (int code : {REPMODE_F32, REPMODE_BF16}) { x[code].reserve(n); numel[code].reserve(n); }
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& t = tensors.get(i);
+    if (t.numel() == 0) continue;
+    if (!t.is_non_overlapping_and_dense()) hold.push_back(t.contiguous());        // (any order of the elements has the same norm)
     const int code = dtype_code(t.scalar_type());
-    x[code].push_back(t.data_ptr());
+    x[code].push_back((t.is_non_overlapping_and_dense() ? t : hold.back()).data_ptr());
     numel[code].push_back((long)t.numel());
-    const long per = REPMODE_GRAD_NORM_CHUNK / t.element_size();
+    const long per = REPMODE_GRAD_NORM_CHUNK / (code == REPMODE_F32 ? 4 : 2);
     room += (t.numel() + per - 1) / per;
   }
-  auto f32 = tensors[0].options().dtype(at::kFloat);
-  Tensor out = at::empty({2}, f32), partial = at::empty({std::max(room, 1L)}, f32.dtype(at::kDouble));
+  auto f32 = tensors.get(0).options().dtype(at::kFloat).requires_grad(false);
+  Tensor norm = at::empty({}, f32), clip = at::empty({}, f32), partial = at::empty({std::max(room, 1L)}, f32.dtype(at::kDouble));
   double* at_ = partial.data_ptr<double>();
   long used = 0;
   for (int code : {REPMODE_F32, REPMODE_BF16})
@@ -1857,59 +1874,75 @@ std::tuple<Tensor, Tensor> op_grad_norm(const std::vector<Tensor>& tensors, doub
       RM_CALL(repmode_grad_norm_partial, cnt, code, x[code].data() + b, numel[code].data() + b, at_ + used, room - used, &n, stream_handle());
       used += n;
     }
-  RM_CALL(repmode_grad_norm_finish, at_, used, max_norm, out.data_ptr<float>(), out.data_ptr<float>() + 1, stream_handle());
-  return {out.select(0, 0), out.select(0, 1)};
+  RM_CALL(repmode_grad_norm_finish, at_, used, max_norm, norm.data_ptr<float>(), clip.data_ptr<float>(), stream_handle());
+  return {norm, clip};
+}
+
+// Whether two of the memory ranges share a byte.  Each list is in the order of its tensors, which mostly is that of their addresses.
+using Spans = std::vector<std::pair<const char*, const char*>>;
+bool overlap(Spans (&lists)[5]) {
+  Spans all, next;
+  for (Spans& l : lists) {
+    if (l.empty()) continue;
+    if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
+    next.resize(all.size() + l.size());
+    std::merge(all.begin(), all.end(), l.begin(), l.end(), next.begin());
+    all.swap(next);
+  }
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].first < all[i - 1].second) return true;
+  return false;
 }
 
 // A parameter's moments are float32 (its scales are not looked at), or 8-bit with one power of two per REPMODE_ADAMW_BLOCK elements
 // in exp_avg_scales / exp_avg_sq_scales; both lists may be empty where no moments are 8-bit.  step_dev: a step that is captured.
-void op_adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs,
-                   const std::vector<Tensor>& exp_avg_scales, const std::vector<Tensor>& exp_avg_sqs,
-                   const std::vector<Tensor>& exp_avg_sq_scales, double lr, double beta1, double beta2, double eps, double weight_decay,
+void op_adamw_step(const TensorList& params, const TensorList& grads, const TensorList& exp_avgs,
+                   const TensorList& exp_avg_scales, const TensorList& exp_avg_sqs,
+                   const TensorList& exp_avg_sq_scales, double lr, double beta1, double beta2, double eps, double weight_decay,
                    int64_t step, const OptTensor& step_dev, const OptTensor& lr_dev, const OptTensor& clip, int64_t seed) {
   const size_t n = params.size();
   TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n && exp_avg_scales.size() == exp_avg_sq_scales.size() &&
                   (exp_avg_scales.empty() || exp_avg_scales.size() == n), "adamw_step: list lengths differ");
   if (n == 0) return;
-  const at::Device dev = params[0].device();
-  std::vector<std::pair<const char*, const char*>> spans;      // what is written
-  spans.reserve(n * (exp_avg_scales.empty() ? 3 : 5));
-  auto span = [&](const Tensor& t) {
-    if (t.numel()) spans.emplace_back(static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes());
+  const at::Device dev = params.get(0).device();
+  Spans written[5];                                            // p, m, v and the two scales: a list each
+  for (Spans& w : written) w.reserve(n);
+  auto span = [&](int list, const Tensor& t) {
+    if (t.numel()) written[list].emplace_back(static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes());
   };
   auto same_order = [](const Tensor& t, const Tensor& p) { return t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous()); };
-  std::vector<char> eight(n);
+  std::vector<char> kind(n);                                   // bit 0: bfloat16, bit 1: 8-bit moments; a kernel each
+  int kinds = 0;
   for (size_t i = 0; i < n; ++i) {
-    const Tensor& p = params[i];
-    const at::ScalarType dt = p.scalar_type();
+    const Tensor &p = params.get(i), &g = grads.get(i), &m = exp_avgs.get(i), &v = exp_avg_sqs.get(i);
+    const at::ScalarType dt = p.scalar_type(), mt = m.scalar_type();
     require_hip(p, "adamw_step: a parameter");
-    (void)dtype_code(dt);
+    const bool eight = mt == at::kFloat8_e4m3fn;
+    kind[i] = (char)((dtype_code(dt) == REPMODE_BF16 ? 1 : 0) | (eight ? 2 : 0));
     TORCH_CHECK(p.device() == dev && p.is_non_overlapping_and_dense(), "adamw_step: parameter ", i, ": dense tensors on one device");
-    TORCH_CHECK(grads[i].layout() == at::kStrided && grads[i].device() == dev && grads[i].scalar_type() == dt && grads[i].sizes() == p.sizes(),
+    TORCH_CHECK(g.layout() == at::kStrided && g.device() == dev && g.scalar_type() == dt && g.sizes() == p.sizes(),
                 "adamw_step: gradient ", i, ": the parameter's type, shape and device");
-    eight[i] = exp_avgs[i].scalar_type() == at::kFloat8_e4m3fn;
-    TORCH_CHECK(exp_avgs[i].scalar_type() == (eight[i] ? at::kFloat8_e4m3fn : at::kFloat) &&
-                    exp_avg_sqs[i].scalar_type() == (eight[i] ? at::kFloat8_e5m2 : at::kFloat),
+    TORCH_CHECK((eight || mt == at::kFloat) && v.scalar_type() == (eight ? at::kFloat8_e5m2 : at::kFloat),
                 "adamw_step: moments of parameter ", i, ": both float32, or float8_e4m3fn and float8_e5m2");
-    for (const Tensor* s : {&exp_avgs[i], &exp_avg_sqs[i]}) {
-      TORCH_CHECK(s->device() == dev && s->sizes() == p.sizes() && same_order(*s, p),
-                  "adamw_step: moments of parameter ", i, ": its shape, strides and device");
-      span(*s);
-    }
-    span(p);
-    if (!eight[i]) continue;
+    TORCH_CHECK(m.device() == dev && m.sizes() == p.sizes() && same_order(m, p) && v.device() == dev && v.sizes() == p.sizes() && same_order(v, p),
+                "adamw_step: moments of parameter ", i, ": its shape, strides and device");
+    if (p.numel() == 0) continue;
+    kinds |= 1 << kind[i];
+    span(0, p);
+    span(1, m);
+    span(2, v);
+    if (!eight) continue;
     TORCH_CHECK(!exp_avg_scales.empty(), "adamw_step: 8-bit moments need their scales");
-    for (const Tensor* s : {&exp_avg_scales[i], &exp_avg_sq_scales[i]}) {
+    const Tensor &ms = exp_avg_scales.get(i), &vs = exp_avg_sq_scales.get(i);
+    for (const Tensor* s : {&ms, &vs})
       TORCH_CHECK(s->device() == dev && s->scalar_type() == at::kFloat8_e8m0fnu && s->is_contiguous() &&
                       s->numel() == (p.numel() + REPMODE_ADAMW_BLOCK - 1) / REPMODE_ADAMW_BLOCK,
                   "adamw_step: scales of parameter ", i, ": one contiguous float8_e8m0fnu value per ", REPMODE_ADAMW_BLOCK, " elements");
-      span(*s);
-    }
+    span(3, ms);
+    span(4, vs);
   }
   // what is written is written once: a tensor given twice, or two views of the same memory, would race
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK(spans[i].first >= spans[i - 1].second, "adamw_step: two of the parameters and moments share memory");
+  TORCH_CHECK(!overlap(written), "adamw_step: two of the parameters and moments share memory");
   auto one = [&](const OptTensor& t, at::ScalarType want, const char* what) {
     if (!t.has_value() || !t->defined()) return;
     TORCH_CHECK(t->device() == dev && t->scalar_type() == want && t->numel() == 1, "adamw_step: ", what, ": one ", want, " value on the parameters' device");
@@ -1925,43 +1958,46 @@ void op_adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>&
   Tensor hyper;
   const float* hd = nullptr;
   if (captured) {
-    hyper = at::empty({REPMODE_ADAMW_HYPER_FLOATS}, params[0].options().dtype(at::kFloat));
+    hyper = at::empty({REPMODE_ADAMW_HYPER_FLOATS}, params.get(0).options().dtype(at::kFloat));
     RM_CALL(repmode_adamw_hyper_dev, reinterpret_cast<long*>(step_dev->data_ptr<int64_t>()), hyper.data_ptr<float>(), lr,
             lr_on_dev ? lr_dev->data_ptr<float>() : nullptr, beta1, beta2, eps, weight_decay, (unsigned long)seed, stream_handle());
     hd = hyper.data_ptr<float>();
   }
   // (also where a launch fails half way: some parameters have changed)
   struct Bump {
-    const std::vector<Tensor>& ps;
+    const TensorList& ps;
     ~Bump() {
-      for (const Tensor& t : ps)
-        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+      for (size_t i = 0; i < ps.size(); ++i)
+        if (const Tensor& t = ps.get(i); !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     }
   } bump{params};
   std::vector<Tensor> hold;                                    // gradients brought into their parameters' order
-  for (int kind = 0; kind < 4; ++kind) {                       // (type of the parameter, bits of the moments): a kernel each
-    const int code = kind & 1 ? REPMODE_BF16 : REPMODE_F32;
+  for (int k = 0; k < 4; ++k) {
+    if (!(kinds >> k & 1)) continue;
+    const bool eight = k & 2;
     void *p[REPMODE_ADAMW_MAX], *m[REPMODE_ADAMW_MAX], *v[REPMODE_ADAMW_MAX], *ms[REPMODE_ADAMW_MAX], *vs[REPMODE_ADAMW_MAX];
     const void* g[REPMODE_ADAMW_MAX];
     long numel[REPMODE_ADAMW_MAX];
     int position[REPMODE_ADAMW_MAX], cnt = 0;
     auto flush = [&]() {
       if (cnt)
-        RM_CALL(repmode_adamw_multi, cnt, code, kind & 2 ? 8 : 32, p, g, m, ms, v, vs, numel, position, lr, beta1, beta2, eps, weight_decay,
-                (long)step, (unsigned long)seed, hd, clip_p, stream_handle());
+        RM_CALL(repmode_adamw_multi, cnt, k & 1 ? REPMODE_BF16 : REPMODE_F32, eight ? 8 : 32, p, g, m, ms, v, vs, numel, position, lr, beta1, beta2,
+                eps, weight_decay, (long)step, (unsigned long)seed, hd, clip_p, stream_handle());
       cnt = 0;
     };
     for (size_t i = 0; i < n; ++i) {
-      if (params[i].numel() == 0 || (bool)eight[i] != (bool)(kind & 2) || dtype_code(params[i].scalar_type()) != code) continue;
-      const void* gp = grads[i].data_ptr();
-      if (!same_order(grads[i], params[i])) {
-        hold.push_back(at::empty_strided(params[i].sizes(), params[i].strides(), grads[i].options()).copy_(grads[i]));
-        gp = hold.back().data_ptr();
-      }
-      p[cnt] = params[i].data_ptr(); g[cnt] = gp; m[cnt] = exp_avgs[i].data_ptr(); v[cnt] = exp_avg_sqs[i].data_ptr();
-      ms[cnt] = eight[i] ? exp_avg_scales[i].data_ptr() : nullptr;
-      vs[cnt] = eight[i] ? exp_avg_sq_scales[i].data_ptr() : nullptr;
-      numel[cnt] = (long)params[i].numel(); position[cnt] = (int)i;
+      const Tensor &pi = params.get(i), &gi = grads.get(i);
+      if (kind[i] != k || pi.numel() == 0) continue;
+      const bool as_is = same_order(gi, pi);
+      if (!as_is) hold.push_back(at::empty_strided(pi.sizes(), pi.strides(), gi.options()).copy_(gi));
+      p[cnt] = pi.data_ptr();
+      g[cnt] = (as_is ? gi : hold.back()).data_ptr();
+      m[cnt] = exp_avgs.get(i).data_ptr();
+      v[cnt] = exp_avg_sqs.get(i).data_ptr();
+      ms[cnt] = eight ? exp_avg_scales.get(i).data_ptr() : nullptr;
+      vs[cnt] = eight ? exp_avg_sq_scales.get(i).data_ptr() : nullptr;
+      numel[cnt] = (long)pi.numel();
+      position[cnt] = (int)i;
       if (++cnt == REPMODE_ADAMW_MAX) flush();
     }
     flush();
@@ -2380,10 +2416,6 @@ TORCH_LIBRARY(repmode, m) {
         "float eps, int step) -> ()", &rm::op_adam_step);
   m.def("adam_step_dev(Tensor[] params, Tensor[] grads, Tensor[] exp_avgs, Tensor[] exp_avg_sqs, float lr, float beta1, float beta2, "
         "float eps, Tensor(a!) step_dev, Tensor(b!) hyper_dev) -> ()", &rm::op_adam_step_dev);
-  m.def("grad_norm(Tensor[] tensors, float max_norm) -> (Tensor, Tensor)", &rm::op_grad_norm);
-  m.def("adamw_step(Tensor[] params, Tensor[] grads, Tensor[] exp_avgs, Tensor[] exp_avg_scales, Tensor[] exp_avg_sqs, "
-        "Tensor[] exp_avg_sq_scales, float lr, float beta1, float beta2, float eps, float weight_decay, int step, Tensor? step_dev, "
-        "Tensor? lr_dev, Tensor? clip, int seed) -> ()", &rm::op_adamw_step);
   m.def("graph_alive(Tensor[] leaves) -> bool", &rm::op_graph_alive);
   m.def("balance_loss(Tensor logits, Tensor? mask, int top_k, float coef) -> (Tensor, Tensor, Tensor)", &rm::op_balance_loss);
   m.def("clear_frag_store() -> ()", &rm::op_clear_frag_store);
@@ -2421,3 +2453,70 @@ TORCH_LIBRARY(repmode, m) {
   m.def("grad_sink_set(Tensor[] params, Tensor[] flats, int[] offsets) -> ()", &rm::op_grad_sink_set);
   m.def("grad_sink_clear() -> ()", &rm::op_grad_sink_clear);
 }
+
+// ------------------------------------------------------------------------------------------------------------
+// The module `librepmode_torch`: grad_norm and adamw_step (repmode_amd/ops.py has their Python faces).
+namespace {
+
+rm::TensorList list_of(PyObject* o, const char* what) {
+  TORCH_CHECK_TYPE(PyList_Check(o) || PyTuple_Check(o), what, ": a list or a tuple of tensors, got ", Py_TYPE(o)->tp_name);
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+  PyObject** items = PySequence_Fast_ITEMS(o);
+  rm::TensorList out;
+  out.t.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    TORCH_CHECK_TYPE(THPVariable_Check(items[i]), what, ": element ", i, " is no tensor but ", Py_TYPE(items[i])->tp_name);
+    out.t.push_back(&THPVariable_Unpack(items[i]));
+  }
+  return out;
+}
+double double_of(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+int64_t int_of(PyObject* o) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+rm::OptTensor optional_of(PyObject* o, const char* what) {
+  if (o == Py_None) return c10::nullopt;
+  TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": a tensor or None, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+
+PyObject* py_grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 2, "grad_norm: 2 arguments, got ", n);
+  auto [norm, clip] = rm::op_grad_norm(list_of(args[0], "grad_norm"), double_of(args[1]));
+  PyObject* out = PyTuple_New(2);
+  if (!out) throw python_error();
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(norm));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(clip));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// (params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, lr, beta1, beta2, eps, weight_decay, step, step_dev, lr_dev,
+//  clip, seed)
+PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 16, "adamw_step: 16 arguments, got ", n);
+  rm::op_adamw_step(list_of(args[0], "params"), list_of(args[1], "grads"), list_of(args[2], "exp_avgs"), list_of(args[3], "exp_avg_scales"),
+                    list_of(args[4], "exp_avg_sqs"), list_of(args[5], "exp_avg_sq_scales"), double_of(args[6]), double_of(args[7]),
+                    double_of(args[8]), double_of(args[9]), double_of(args[10]), int_of(args[11]), optional_of(args[12], "step"),
+                    optional_of(args[13], "lr"), optional_of(args[14], "clip"), int_of(args[15]));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef g_methods[] = {
+    {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_grad_norm)), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_adamw_step)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "librepmode_torch", nullptr, -1, g_methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_librepmode_torch() { return PyModule_Create(&g_module); }

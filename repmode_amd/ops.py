@@ -61,6 +61,18 @@ def torch_ops():
     return _TOPS
 
 
+_LIST_OPS = None
+
+
+def list_ops():
+    """The operators over lists of hundreds of tensors (``grad_norm``, ``adamw_step``): the operator library's own module, whose
+    functions read a Python list as it is (the dispatcher behind ``torch.ops`` boxes every tensor of one)."""
+    global _LIST_OPS
+    if _LIST_OPS is None:
+        _LIST_OPS = _lib.load_list_ops()
+    return _LIST_OPS
+
+
 # ---- a second HIP stream for independent launches of one layer.  On the deep levels a conv / filter-gradient launch
 # has 128-256 workgroups for 512 slots, and a layer's data gradient, filter gradient and 1x1-expert GEMMs do not depend
 # on each other: issued on two streams they share the chip instead of queueing behind each other's tails
@@ -384,7 +396,7 @@ def grad_norm(tensors, max_norm=None):
     order) and the factor ``min(1, max_norm / (norm + 1e-6))`` that clips them, both float32 scalars on the device -- no
     synchronisation, nothing is scaled here.  ``clip`` is NaN where the norm is not finite (``adamw_step`` then leaves the
     step out); without ``max_norm`` it is 1.  No autograd."""
-    return torch_ops().grad_norm(list(tensors), float('inf') if max_norm is None else float(max_norm))
+    return list_ops().grad_norm(list(tensors), float('inf') if max_norm is None else float(max_norm))
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, clip=None, seed=0):
@@ -405,9 +417,9 @@ def adamw8_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq
     (``adamw8_state`` makes them).  The arithmetic is float32; what is kept is rounded stochastically.  A tensor whose moments
     are float32 is updated as ``adamw_step`` does (its scales are not looked at): one list may hold both kinds."""
     on_device, lr_on_device = torch.is_tensor(step), torch.is_tensor(lr)
-    torch_ops().adamw_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, 0.0 if lr_on_device else float(lr),
-                           float(betas[0]), float(betas[1]), float(eps), float(weight_decay), 0 if on_device else int(step),
-                           step if on_device else None, lr if lr_on_device else None, clip, int(seed))
+    list_ops().adamw_step(params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, 0.0 if lr_on_device else float(lr),
+                          float(betas[0]), float(betas[1]), float(eps), float(weight_decay), 0 if on_device else int(step),
+                          step if on_device else None, lr if lr_on_device else None, clip, int(seed))
 
 
 def adamw8_state(param):

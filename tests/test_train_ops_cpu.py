@@ -29,6 +29,13 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match='list lengths'):
         ops.adamw_step([x], [], [x], [x], 1)
     ops.adamw_step([], [], [], [], 1)                    # (nothing to do)
+    for bad in ([1], [None], x, 'x', None):
+        with pytest.raises(TypeError):
+            ops.adamw_step([x], bad, [x], [x], 1)
+    with pytest.raises(TypeError, match='no tensor'):
+        ops.grad_norm([x, 3])
+    with pytest.raises(TypeError, match='clip'):
+        ops.adamw_step([x], [x], [x], [x], 1, clip=0.5)
 
 
 def test_adamw8_state_layout():
@@ -143,7 +150,7 @@ def test_adamw_bookkeeping(monkeypatch):
     number of updates they have seen."""
     from repmode_amd import ops, optim
     fake = _FakeOps()
-    monkeypatch.setattr(ops, 'torch_ops', lambda: fake)
+    monkeypatch.setattr(ops, 'list_ops', lambda: fake)
     big, small, other = (torch.nn.Parameter(torch.randn(n)) for n in (5000, 7, 9000))
     opt = optim.AdamW([dict(params=[big, small]), dict(params=[other], weight_decay=0.0, state_bits=32)], lr=2e-3, max_norm=1.5, state_bits=8, seed=9)
     for p in (big, small, other):
@@ -169,7 +176,7 @@ def test_adamw_state_dicts(monkeypatch, tmp_path):
     """8-bit moments and the float32 moments of bfloat16 parameters survive save / load as they are; float32 states
     interchange with torch.optim.AdamW's."""
     from repmode_amd import ops, optim
-    monkeypatch.setattr(ops, 'torch_ops', lambda: _FakeOps())
+    monkeypatch.setattr(ops, 'list_ops', lambda: _FakeOps())
     make = lambda: [torch.nn.Parameter(torch.zeros(n, dtype=d)) for n, d in ((5000, torch.bfloat16), (300, torch.bfloat16), (20, torch.float32))]
     ps, qs = make(), make()
     opt, back = optim.AdamW(ps, state_bits=8), optim.AdamW(qs)
