@@ -77,7 +77,7 @@ static_assert(sizeof(AdamWArgs) <= 4096, "launch arguments");
 // (4 / 32 / 128 M float32 parameters, float32 moments: 24.6 / 162 / 640 us, through the caches 32.0 / 184 / 706; right after the norm
 // of the same gradients 20.7 / 144 / 603 and 25.0 / 160 / 663.  Only a list of tens of MB that is updated again and again with nothing
 // in between would gain by the caches: 28.3 and 26.1 at 4 M.)
-enum { AW_PART = 0, AW_WHOLE = 1 };
+enum { AW_PART = 0, AW_WHOLE = 1, AW_SOME = 2 };
 template <typename V>
 __device__ __forceinline__ V fetch(const V* p) { return __builtin_nontemporal_load(p); }
 template <typename V>
@@ -285,7 +285,8 @@ __device__ __forceinline__ void encode4(const f32x4& m, const f32x4& v, const ui
   }
 }
 
-// UNITS blocks of each wave; all their loads are under way before the first is used.
+// UNITS blocks of each wave (AW_SOME: those of them that lie in the tensor as a whole); all their loads are under way before the first
+// is used.
 template <typename T, bool EIGHT, int HOW, int UNITS>
 __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const AdamWHyper& h, float clip, uint32_t key, long chunk, int unit, int wave,
                                             int lane, long n) {
@@ -299,6 +300,7 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
   for (int u = 0; u < UNITS; ++u) {
     const long o = chunk + ((unit + u) * AW_WAVES + wave) * AW_BLOCK;         // of the wave's block; uniform
     const int left = HOW != AW_PART ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
+    if (HOW == AW_SOME && o + AW_BLOCK > n) break;
     P[u] = load4<HOW>(static_cast<const T*>(a.p[i]) + o + lane * 4, left);
     G[u] = load4<HOW>(static_cast<const T*>(a.g[i]) + o + lane * 4, left);
     M[u] = load4<HOW>(static_cast<const S*>(a.m[i]) + o + lane * 4, left);
@@ -308,11 +310,13 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
       VE[u] = a.vs[i][o / AW_BLOCK];
     }
   }
+  if (clip != clip) return;                                    // gradients that are not finite: the step is left out
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
     const int j = ((unit + u) * AW_WAVES + wave) * AW_BLOCK + lane * 4;
     const long o = chunk + ((unit + u) * AW_WAVES + wave) * AW_BLOCK;
     const int left = HOW != AW_PART ? 4 : (int)(n - o < AW_BLOCK ? n - o : AW_BLOCK) - lane * 4;
+    if (HOW == AW_SOME && o + AW_BLOCK > n) break;
     T* p = static_cast<T*>(a.p[i]) + o + lane * 4;
     S* m = static_cast<S*>(a.m[i]) + o + lane * 4;
     S* v = static_cast<S*>(a.v[i]) + o + lane * 4;
@@ -346,9 +350,11 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
 
 template <typename T, bool EIGHT>
 __global__ __launch_bounds__(64 * AW_WAVES) void adamw_kernel(AdamWArgs a) {
-  const float clip = a.clip ? *a.clip : 1.f;
-  if (clip != clip) return;                                   // gradients that are not finite: the step is left out
-  const AdamWHyper h = a.hd ? *a.hd : a.h;
+  float clip = 1.f;
+  if (a.clip) clip = *a.clip;
+  AdamWHyper h = a.h;
+  if (a.hd) h = *a.hd;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int i = 0;
   for (int hi = a.nt; hi - i > 1;) {                           // the tensor of this workgroup: first[i] <= blockIdx.x < first[i + 1]
     const int mid = (i + hi) >> 1;
@@ -356,24 +362,25 @@ __global__ __launch_bounds__(64 * AW_WAVES) void adamw_kernel(AdamWArgs a) {
     else hi = mid;
   }
   const long n = a.numel[i];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long chunk = (long)((int)blockIdx.x - a.first[i]) * AW_CHUNK;
   // (a chunk never crosses a multiple of 2^32: the upper half of the element index is the workgroup's)
   uint32_t key = mix32(h.base + (uint32_t)a.position[i]);
   if (chunk >> 32) key = mix32(key + (uint32_t)(chunk >> 32));
   constexpr uintptr_t PA = 4 * sizeof(T) - 1, SA = EIGHT ? 3 : 15;
   const bool aligned = (((uintptr_t)a.p[i] | (uintptr_t)a.g[i]) & PA) == 0 && (((uintptr_t)a.m[i] | (uintptr_t)a.v[i]) & SA) == 0;
-  if (aligned && chunk + AW_CHUNK <= n) {
+  if (!aligned) {
+#pragma unroll 1
+    for (int u = 0; u < AW_UNITS; ++u)
+      if (chunk + (u * AW_WAVES + wave) * AW_BLOCK < n) adamw_units<T, EIGHT, AW_PART, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
+    return;
+  }
+  if (chunk + AW_CHUNK <= n) {
     adamw_units<T, EIGHT, AW_WHOLE, AW_UNITS>(a, i, h, clip, key, chunk, 0, wave, lane, n);
     return;
   }
-#pragma unroll 1
-  for (int u = 0; u < AW_UNITS; ++u) {
-    const long o = chunk + (u * AW_WAVES + wave) * AW_BLOCK;
-    if (o >= n) break;
-    if (aligned && o + AW_BLOCK <= n) adamw_units<T, EIGHT, AW_WHOLE, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
-    else adamw_units<T, EIGHT, AW_PART, 1>(a, i, h, clip, key, chunk, u, wave, lane, n);
-  }
+  adamw_units<T, EIGHT, AW_SOME, AW_UNITS>(a, i, h, clip, key, chunk, 0, wave, lane, n);
+  const int whole = (int)((n - chunk) / AW_BLOCK);             // the block behind them, if the tensor ends inside it
+  if ((n - chunk) % AW_BLOCK && whole % AW_WAVES == wave) adamw_units<T, EIGHT, AW_PART, 1>(a, i, h, clip, key, chunk, whole / AW_WAVES, wave, lane, n);
 }
 
 int check_hyper(double lr, double beta1, double beta2, double eps, double weight_decay) {

@@ -487,12 +487,18 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs 
     for (int j = 1; j < EPL; ++j) top = max(top, key_of(x[j]));
     const float sum = row_exp<LPR>(top_of<float>(row_max<LPR>(top)), x, x);
     const float inv = sum != 0.f ? __builtin_amdgcn_rcpf(sum) : 0.f;
-    float dot = 0.f;
+    // w_e - d with d = sum_j w_j p_j, which is (w_e - r) - sum_j (w_j - r) p_j for any r, the sum of the p_j being 1.  With d's first
+    // value for r the second sum is what that value was off by, and neither the rounding of the p_j's sum nor that of a p_j near 1
+    // is left in the differences: for a row that one expert has nearly to itself they are as small as what the others have.
+    float r = 0.f, d = 0.f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) { x[j] *= inv; dot += x[j] * w[j]; }
-    dot = row_sum<LPR>(dot);
+    for (int j = 0; j < EPL; ++j) { x[j] *= inv; r = fmaf(x[j], w[j], r); }
+    r = row_sum<LPR>(r);
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) x[j] = sum != 0.f ? x[j] * (w[j] - dot) : 0.f;      // (a row that does not count: 0 whatever w is)
+    for (int j = 0; j < EPL; ++j) d = fmaf(x[j], w[j] - r, d);
+    d = row_sum<LPR>(d);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) x[j] = sum != 0.f ? x[j] * ((w[j] - r) - d) : 0.f;      // (a row that does not count: 0 whatever w is)
   };
   if constexpr (TILED) {
     extern __shared__ float tile[];

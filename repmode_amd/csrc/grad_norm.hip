@@ -48,21 +48,29 @@ template <typename T>
 __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(NormArgs a, double* __restrict__ partial) {
   constexpr int VEC = 16 / sizeof(T), ITEMS = GN_CHUNK / 16 / GN_THREADS;
   int i = 0;
-  for (int lo = 0, hi = a.nt; hi - lo > 1;) {
-    const int mid = (lo + hi) >> 1;
-    if ((int)blockIdx.x >= a.first[mid]) lo = mid;
+  for (int hi = a.nt; hi - i > 1;) {                           // the tensor of this workgroup: first[i] <= blockIdx.x < first[i + 1]
+    const int mid = (i + hi) >> 1;
+    if ((int)blockIdx.x >= a.first[mid]) i = mid;
     else hi = mid;
-    i = lo;
   }
   const long base = (long)((int)blockIdx.x - a.first[i]) * (GN_CHUNK / sizeof(T)), n = a.numel[i];
   const T* __restrict__ x = static_cast<const T*>(a.x[i]);
   double sum = 0;
   auto add = [&](float f) { sum = fma((double)f, (double)f, sum); };
-  if (((uintptr_t)x & 15) == 0 && base + (long)(GN_CHUNK / sizeof(T)) <= n) {
+  const long end = base + (long)(GN_CHUNK / sizeof(T)) < n ? base + (long)(GN_CHUNK / sizeof(T)) : n;
+  long rest = base;                                             // what is left to take one by one
+  if (((uintptr_t)x & 15) == 0) {
+    const int pieces = (int)(end - base) / VEC;                 // of 16 bytes; all loads are under way before the first is used
     const u32x4* q = reinterpret_cast<const u32x4*>(x + base) + threadIdx.x;
     u32x4 w[ITEMS];
+    if (pieces == ITEMS * GN_THREADS) {
 #pragma unroll
-    for (int u = 0; u < ITEMS; ++u) w[u] = __builtin_nontemporal_load(q + u * GN_THREADS);
+      for (int u = 0; u < ITEMS; ++u) w[u] = __builtin_nontemporal_load(q + u * GN_THREADS);
+    } else {
+#pragma unroll
+      for (int u = 0; u < ITEMS; ++u) w[u] = u * GN_THREADS + (int)threadIdx.x < pieces ? q[u * GN_THREADS] : u32x4{0, 0, 0, 0};
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < ITEMS; ++u)
 #pragma unroll
@@ -74,10 +82,9 @@ __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(NormArgs a, doubl
           add(__uint_as_float(w[u][k] & 0xffff0000u));
         }
       }
-  } else {
-    const long end = base + (long)(GN_CHUNK / sizeof(T)) < n ? base + (long)(GN_CHUNK / sizeof(T)) : n;
-    for (long o = base + threadIdx.x; o < end; o += GN_THREADS) add(to_f32<T>(x[o]));
+    rest += (long)pieces * VEC;
   }
+  for (long o = rest + threadIdx.x; o < end; o += GN_THREADS) add(to_f32<T>(x[o]));
   sum = block_sum<GN_THREADS>(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
