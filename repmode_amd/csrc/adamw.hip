@@ -17,7 +17,10 @@
 // tensor's position, element), so a run repeats itself bit by bit.  A v above zero is never rounded to zero: m / (0 + eps)
 // would throw its parameter away.  What is not finite stays so (e4m3 has no infinity: NaN) and is left out of the block's scale.
 //
-// What bounds both: HBM.  float32 moments move 28 B an element (bfloat16 parameters: 22), 8-bit ones 16 (10).
+// What bounds both: HBM.  float32 moments move 28 B an element (bfloat16 parameters: 22), 8-bit ones 16 (10).  108.6 M float32 parameters
+// 517 us (5.9 TB/s; four reads and three writes without arithmetic reach that too) and, 8-bit moments, 283 us (6.1); 201 M bfloat16
+// ones 755 us (5.9), 402.8 M with 8-bit moments 697 us (5.8).  With bfloat16 parameters and 8-bit moments the vector units are next:
+// hence one hash multiplication for four elements, and the hardware's stochastic conversions.
 #include "common.h"
 
 #include <cmath>

@@ -18,7 +18,9 @@
 //   A workgroup walks many rows and writes one partial per expert; one launch adds the partials of a group's columns in a fixed
 // order in float64, one more makes the loss of them; where one workgroup has seen all rows it does both itself.  No float atomics: a
 // run repeats itself bit by bit.  The backward pass reads the logits again and needs nothing of a row but its logits.
-// What bounds it: HBM for the backward pass (one read, one write), the instructions of exponential and choice for forward passes.
+// What bounds it: the backward pass HBM (one read, one write: 262144 x 256 float32 logits 84 us, 6.4 TB/s), the forward pass the
+// instructions of exponential and choice (the same logits 67 us for the top 1, 83 for the top 8 and 9 for the columns, where a read
+// takes 40).
 #include "common.h"
 
 #include <atomic>
@@ -78,16 +80,17 @@ __device__ __forceinline__ int row_max(int v) { return over_row<LPR>(v, [](int a
 template <int LPR, typename T>
 __device__ __forceinline__ T row_sum(T v) { return over_row<LPR>(v, [](T a, T b) { return a + b; }); }
 
-// Integers in the order of the floats: negative ones with their magnitude turned over.  x + 0 makes -0 a 0.  What lies below NOT_LOWEST
-// is -inf (or a NaN with its sign bit); a NaN without it lies above all.
-constexpr int NOT_LOWEST = (int)0x80800000;
-__device__ __forceinline__ int turn(int u) { return u ^ ((u >> 31) & 0x7fffffff); }
-__device__ __forceinline__ int key_of(float x) { return turn(__float_as_int(x + 0.f)); }
-// the softmax's shift of a row whose largest key this is (a lower half that holds an index is none of the value's)
+// Integers in the order of the floats: a negative float's is its magnitude's, negated, so -0 and 0 have one key.  What lies below
+// not_lowest is -inf (or a NaN with its sign bit); a NaN without it lies above all.  The same step leads back.
+__device__ __forceinline__ int turn(int u) { return u < 0 ? (int)0x80000000 - u : u; }
+// (a bfloat16 value's key leaves the lower half to the index)
+template <typename T>
+constexpr int not_lowest = sizeof(T) == 2 ? (int)0x80810000 : (int)0x80800001;
+// the softmax's shift of a row whose largest key this is
 template <typename T>
 __device__ __forceinline__ float top_of(int key) {
-  if (key < NOT_LOWEST) return 0.f;                          // (nothing but -inf)
-  return __int_as_float(sizeof(T) == 2 ? turn(key) & (int)0xffff0000 : turn(key));
+  if (key < not_lowest<T>) return 0.f;                       // (nothing but -inf)
+  return __int_as_float(turn(sizeof(T) == 2 ? key & (int)0xffff0000 : key));
 }
 
 // y_j = e^(x_j - top) of a row (y may be x), and its sum.  As 2^(x_j L - top L), L = log2(e), in one fused step: the rounding of
@@ -228,16 +231,28 @@ __device__ __forceinline__ void row_of_tile(const BalanceArgs& a, const float* t
 // cnt += the lane's chosen values of a row: those of at least the k-th largest key t
 template <typename T, int LPR, int EPL, int V>
 __device__ __forceinline__ void choose(const int (&key)[EPL], int t, int sub, int top_k, int (&cnt)[EPL]) {
-  const int from = max(t, NOT_LOWEST);
+  const int from = max(t, not_lowest<T>);
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) cnt[j] += key[j] >= from;
   } else {
+    // A row with top_k values or more has at least top_k of t or more, and equal ones only if it has more.  Over the wave's rows by
+    // ballots; where a row has fewer, row by row.
     bool in[EPL];
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) { in[j] = key[j] >= from; n += in[j]; }
-    if (__any(row_sum<LPR>(n) > top_k)) {                     // equal values: one by one, the largest that is left, the lowest index first
+    for (int j = 0; j < EPL; ++j) {
+      in[j] = key[j] >= from;
+      n += __popcll(__ballot(in[j]));
+    }
+    bool equal = n != 64 / LPR * top_k || __any(t < not_lowest<T>);
+    if (equal) {
+      int own = 0;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) own += in[j];
+      equal = __any(row_sum<LPR>(own) > top_k);
+    }
+    if (equal) {                                              // one by one, the largest that is left, the lowest index first
       int s[EPL];
 #pragma unroll
       for (int j = 0; j < EPL; ++j) s[j] = key[j];
@@ -249,7 +264,7 @@ __device__ __forceinline__ void choose(const int (&key)[EPL], int t, int sub, in
         int at = -BL_MAX_E;
 #pragma unroll
         for (int j = EPL - 1; j >= 0; --j)
-          if (s[j] == best && best >= NOT_LOWEST) at = -expert_of<LPR, V>(j, sub);
+          if (s[j] == best && best >= not_lowest<T>) at = -expert_of<LPR, V>(j, sub);
         at = -row_max<LPR>(at);
 #pragma unroll
         for (int j = 0; j < EPL; ++j)
@@ -309,8 +324,8 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
     int key[EPL], s[EPL];
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      key[j] = key_of(x[j]);
-      if constexpr (sizeof(T) == 2) key[j] = (key[j] & (int)0xffff0000) | (0xffff - expert_of<LPR, V>(j, sub));
+      key[j] = turn(__float_as_int(x[j]));
+      if constexpr (sizeof(T) == 2) key[j] |= 0xffff - expert_of<LPR, V>(j, sub);
       s[j] = key[j];
     }
     sort_descending(s);
@@ -337,22 +352,31 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
     }
   } else {
     const long step = (long)a.blocks * BL_WAVES * RPW;
-    float next[EPL];
+    float x[EPL], next[EPL];
     long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW;
     const T* row = x0 + (n0 + slot) * a.sn;
     long masked = (n0 + slot) * a.mn;
-    auto fetch = [&](long n) {
-      load_row<T, LPR, EPL, V>(a, row, n < a.rows && (!mask || mask[masked]), sub, next);
+    auto fetch = [&](float (&to)[EPL], long n) {
+      load_row<T, LPR, EPL, V>(a, row, n < a.rows && (!mask || mask[masked]), sub, to);
       row += step * a.sn;
       masked += step * a.mn;
     };
-    if (n0 < a.rows) fetch(n0 + slot);
-    for (; n0 < a.rows; n0 += step) {
-      float x[EPL];
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) x[j] = next[j];
-      if (n0 + step < a.rows) fetch(n0 + step + slot);      // (under way while this row is worked on)
+    // A row is fetched while the one before it is worked on.  Two sets of registers take turns; with 16 values a lane the second copy of
+    // the work costs more registers than it saves moves (1024 experts: 97 us, with moves 88; 256: 68 and 76).
+    if (n0 < a.rows) fetch(x, n0 + slot);
+    while (n0 < a.rows) {
+      n0 += step;
+      if (n0 < a.rows) fetch(next, n0 + slot);
       work(x);
+      if (n0 >= a.rows) break;
+      if constexpr (EPL > 8) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) x[j] = next[j];
+      } else {
+        n0 += step;
+        if (n0 < a.rows) fetch(x, n0 + slot);
+        work(next);
+      }
     }
   }
   // the wave's rows, then the workgroup's waves
@@ -482,9 +506,9 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs 
     w[j] = e < a.experts ? scale * a.weight[(long)g * a.experts + e] : 0.f;
   }
   auto work = [&](float (&x)[EPL]) {                        // logits in, gradients out
-    int top = key_of(x[0]);
+    int top = turn(__float_as_int(x[0]));
 #pragma unroll
-    for (int j = 1; j < EPL; ++j) top = max(top, key_of(x[j]));
+    for (int j = 1; j < EPL; ++j) top = max(top, turn(__float_as_int(x[j])));
     const float sum = row_exp<LPR>(top_of<float>(row_max<LPR>(top)), x, x);
     const float inv = sum != 0.f ? __builtin_amdgcn_rcpf(sum) : 0.f;
     // w_e - d with d = sum_j w_j p_j, which is (w_e - r) - sum_j (w_j - r) p_j for any r, the sum of the p_j being 1.  With d's first

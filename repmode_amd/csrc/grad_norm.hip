@@ -5,7 +5,7 @@
 // gradients of 1e-30 and of 1e30 count for what they are; the float64 units keep up with HBM (one conversion and one fused
 // multiply-add an element).  The sum's order is fixed -- a workgroup per GN_CHUNK bytes of a tensor, one partial each, the
 // partials added by one workgroup in a fixed order -- so a run repeats itself bit by bit.
-// What bounds it: HBM, one read of the tensors, past the caches: 64 / 256 M float32 values 48 / 161 us (5.6 / 6.7 TB/s), through them 91 /
+// What bounds it: HBM, one read of the tensors, past the caches: 64 / 256 M float32 values 47 / 165 us (5.7 / 6.5 TB/s), through them 91 /
 // 246 us -- and an update that reads the gradients next gains less by finding a part of them there than the norm loses (norm and
 // update of 128 M float32 values 716 and 739 us).
 #include "common.h"
