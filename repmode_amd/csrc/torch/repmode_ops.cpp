@@ -2030,6 +2030,7 @@ struct BalanceLoss : public torch::autograd::Function<BalanceLoss> {
     auto sv = ctx->get_saved_variables();
     const Tensor &x = sv[0], &mask = sv[1], &weight = sv[2];
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    TORCH_CHECK(!at::GradMode::is_enabled(), "balance_loss: no second derivative (create_graph=True)");
     DeviceGuard guard(x.device());
     const bool grouped = x.dim() == 3, masked = mask.defined();
     const int64_t groups = grouped ? x.size(0) : 1, rows = x.size(-2), experts = x.size(-1);

@@ -246,7 +246,8 @@ class Net(torch.nn.Module):
         for m in self.modules():
             if isinstance(m, MoDEConv):
                 # (experts the slowest axis, as the gate lays them out: RepMode.py:198-200)
-                logits = torch.addmm(m.gate.bias[:, None], m.gate.weight, onehot).view(NUM_EXPERTS, -1).t()
+                with torch.autocast(device.type, enabled=False):
+                    logits = torch.addmm(m.gate.bias[:, None], m.gate.weight, onehot).view(NUM_EXPERTS, -1).t()
                 loss, count, prob = ops.balance_loss(logits, top_k, coef=coef)
                 losses.append(loss)
                 counts.append(count)

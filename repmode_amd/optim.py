@@ -63,6 +63,8 @@ class Adam(torch.optim.Adam):
     def load_state_dict(self, state_dict):
         """As torch.optim.Adam; `step` counters that a fused / capturable optimizer kept on the device come to the host (one
         copy at load time, so that ``step()`` never reads the device to learn the step count)."""
+        if any('exp_avg_scale' in st for st in state_dict['state'].values()):
+            raise ValueError('repmode_amd.optim.Adam: these moments are in 8 bits (optim.AdamW)')
         super().load_state_dict(state_dict)
         for group in self.param_groups:            # (a stock optimizer's groups say fused / capturable; this one's bookkeeping is neither)
             group['fused'], group['capturable'], group['foreach'] = False, False, False
@@ -127,6 +129,10 @@ class Adam(torch.optim.Adam):
         return loss
 
 
+def _capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) over all tensors at once, with the gradients clipped by their common norm in the same step
     and the moments in float32 or in 8 bits (csrc/adamw.hip, csrc/grad_norm.hip).  float32 and bfloat16 parameters.
@@ -161,10 +167,18 @@ class AdamW(torch.optim.Optimizer):
             bits = self.param_groups.pop()['state_bits']
             raise ValueError('repmode_amd.optim.AdamW: moments in 8 or 32 bits, got %r' % (bits,))
 
+    def __getstate__(self):
+        self.sync_steps()
+        return {**super().__getstate__(), 'max_norm': self.max_norm, 'seed': self.seed, 'device_step': self.device_step, 'last_norm': None,
+                '_step_dev': {}}
+
     def _state(self, p, group):
         st = self.state[p]
         if not st:
             from . import ops as ops_
+            if self.device_step and _capturing():
+                # (the zeros would be part of the graph, and every replay begin with them)
+                raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): a parameter\'s first step must not be a captured one')
             st['step'] = torch.tensor(0.0)
             if group['state_bits'] == 8 and p.numel() >= group['min_8bit_numel']:
                 st['exp_avg'], st['exp_avg_scale'], st['exp_avg_sq'], st['exp_avg_sq_scale'] = ops_.adamw8_state(p)
@@ -187,6 +201,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel')} for g in self.param_groups]
+        # (captured steps hold the moments by address, as they do the step counts: what fits goes into the tensors that are there)
+        held = {p: dict(st) for p, st in self.state.items()} if self.device_step else {}
         super().load_state_dict(state_dict)
         for group, mine in zip(self.param_groups, own):          # (a stock optimizer's groups have neither)
             for k, v in mine.items():
@@ -200,8 +216,12 @@ class AdamW(torch.optim.Optimizer):
                         self.state[p][k] = torch.tensor(float(v))
                     elif torch.is_tensor(v):
                         v = v.detach().to(p.device, copy=True)
-                        self.state[p][k] = v.float() if v.dtype in (torch.bfloat16, torch.float16) else v
-        for gi, dev in list(self._step_dev.items()):             # (captured steps hold the counts by address: in place)
+                        v = v.float() if v.dtype in (torch.bfloat16, torch.float16) else v
+                        there = held.get(p, {}).get(k)
+                        if torch.is_tensor(there) and there.dtype == v.dtype and there.shape == v.shape:
+                            v = there.copy_(v)
+                        self.state[p][k] = v
+        for gi, dev in list(self._step_dev.items()):
             counts = {int(self.state[p]['step']) for p in self.param_groups[gi]['params'] if 'step' in self.state.get(p, {})}
             if len(counts) <= 1:
                 dev.fill_(counts.pop() if counts else 0)
@@ -214,7 +234,7 @@ class AdamW(torch.optim.Optimizer):
             t0 = {int(s) for s in steps}
             if len(t0) != 1:
                 raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): the parameters of a group must have seen the same number of steps')
-            if torch.cuda.is_current_stream_capturing():
+            if _capturing():
                 raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): run one step launch by launch before capturing')
             self._step_dev[gi] = torch.full((1,), t0.pop(), dtype=torch.int64, device=device)
         for s in steps:
@@ -240,6 +260,8 @@ class AdamW(torch.optim.Optimizer):
                 grads += [p.grad for p in ps]
         if not work:
             return loss
+        if not self.device_step and _capturing():
+            raise RuntimeError('repmode_amd.optim.AdamW: a captured step needs capturable=True')
         clip = None
         if self.max_norm is not None:
             self.last_norm, clip = ops_.grad_norm(grads, self.max_norm)

@@ -9,11 +9,12 @@ from test_hip_parity import _ops
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize('kw', [{}, dict(optimizer='adamw', optimizer_args=dict(max_norm=0.1, state_bits=8), balance_coef=0.25)])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
-def test_every_replay_has_the_eager_gradients(dtype):
+def test_every_replay_has_the_eager_gradients(dtype, kw):
     from repmode_amd.model import Model
     _ops()
-    make = lambda graph: Model(Opts(), lr=1e-3, gpu_ids=0, mult_chan=4, dtype=dtype, hip_graph=graph)
+    make = lambda graph: Model(Opts(), lr=1e-3, gpu_ids=0, mult_chan=4, dtype=dtype, hip_graph=graph, **kw)
     torch.manual_seed(0)
     m, e = make(True), make(False)
     gen = torch.Generator().manual_seed(1)

@@ -217,6 +217,35 @@ def test_adamw_state_dicts(monkeypatch, tmp_path):
     assert float(again.state[r[0]]['step']) == 3.0
 
 
+def test_adamw_copies(monkeypatch):
+    """copy.deepcopy (pickle's way) keeps the settings; 8-bit moments are refused by the plain Adam."""
+    import copy
+    from repmode_amd import ops, optim
+    monkeypatch.setattr(ops, 'list_ops', lambda: _FakeOps())
+    p = torch.nn.Parameter(torch.zeros(5000))
+    opt = optim.AdamW([p], max_norm=2.0, state_bits=8, seed=7)
+    p.grad = torch.ones(5000)
+    opt.step()
+    other = copy.deepcopy(opt)
+    q = other.param_groups[0]['params'][0]
+    assert other.max_norm == 2.0 and other.seed == 7 and other.device_step is False and other.state[q]['exp_avg'].dtype == torch.float8_e4m3fn
+    q.grad = torch.ones(5000)
+    other.step()
+    assert int(other.state[q]['step']) == 2 and int(opt.state[p]['step']) == 1
+    with pytest.raises(ValueError, match='8 bits'):
+        optim.Adam([p]).load_state_dict(opt.state_dict())
+
+
+def test_list_ops_arguments():
+    ops = _ops()
+    with pytest.raises(TypeError, match='16 arguments'):
+        ops.list_ops().adamw_step([])
+    with pytest.raises(TypeError):
+        ops.list_ops().grad_norm([torch.zeros(1)], 'x')
+    with pytest.raises(TypeError):
+        ops.list_ops().adamw_step([], [], [], [], [], [], 1e-3, 0.9, 0.99, 1e-8, 0.0, 'x', None, None, None, 0)
+
+
 def test_graph_alive_sees_a_held_graph():
     ops = _ops()
     p = torch.nn.Parameter(torch.ones(3))

@@ -151,7 +151,7 @@ def test_balance_loss_empty_groups():
         y = y.detach().requires_grad_(True)
         loss, counts, prob = ops.balance_loss(y, 2, mask=m)
         grad, = torch.autograd.grad(loss, y)
-        assert float(loss) == 0 and int(counts.sum()) == 0 and float(prob.sum()) == 0 and float(grad.abs().sum()) == 0
+        assert float(loss.detach()) == 0 and int(counts.sum()) == 0 and float(prob.sum()) == 0 and float(grad.abs().sum()) == 0
 
 
 def test_balance_loss_not_finite():
@@ -194,6 +194,31 @@ def test_balance_loss_checks():
                        (lambda: ops.balance_loss(torch.zeros(1, 1025, device=DEV), 1), 'experts'), (lambda: ops.balance_loss(x[:0], 1), 'groups')):
         with pytest.raises(RuntimeError, match=says):
             call()
+
+
+def test_balance_loss_autograd_limits():
+    """Logits or mask changed in place after the forward pass, and a second derivative, are errors; two backward passes are not."""
+    ops = _ops()
+    x = torch.randn(40, 12, device=DEV, requires_grad=True)
+    mask = torch.ones(40, dtype=torch.bool, device=DEV)
+    loss = ops.balance_loss(x, 2, mask=mask)[0]
+    a, = torch.autograd.grad(loss, x, retain_graph=True)
+    b, = torch.autograd.grad(loss, x, retain_graph=True)
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(loss, x, create_graph=True)
+    mask[3] = False
+    with pytest.raises(RuntimeError, match='modified by an inplace'):
+        torch.autograd.grad(loss, x)
+    loss = ops.balance_loss(x, 2)[0]
+    with torch.no_grad():
+        x += 1
+    with pytest.raises(RuntimeError, match='modified by an inplace'):
+        torch.autograd.grad(loss, x)
+    counts, prob = ops.balance_loss(x, 2)[1:]
+    assert not counts.requires_grad and not prob.requires_grad
+    y = x.detach().expand(3, 40, 12)
+    _check_balance(y, 2)
 
 
 def test_balance_loss_repeats_itself_on_any_stream():
@@ -685,6 +710,76 @@ def test_adamw_in_a_graph(bits):
         assert int(count) == t and torch.equal(norm, want)
         for x, y in zip(a[0] + sum(a[2], []), b[0] + sum(b[2], [])):
             assert torch.equal(_bytes(x), _bytes(y)), t
+
+
+def test_adamw_optimizer_in_a_graph():
+    """optim.AdamW(capturable=True): two groups (8- and 32-bit moments, one learning rate on the device) captured and replayed against a
+    twin that steps launch by launch; a state loaded in between goes into the tensors that the graph holds; what a capture must not
+    hold is refused."""
+    import copy
+    from repmode_amd.optim import AdamW
+    _ops()
+    def make(capturable):
+        ps = [torch.nn.Parameter(torch.randn(n, generator=torch.Generator().manual_seed(n)).to(DEV)) for n in (5000, 300, 9000)]
+        lr = torch.tensor(1e-2, device=DEV) if capturable else 1e-2
+        return ps, AdamW([dict(params=ps[:2], state_bits=8), dict(params=ps[2:], lr=lr)], lr=2e-3, max_norm=1.0, capturable=capturable, seed=4)
+    (ps, opt), (qs, twin) = make(True), make(False)
+    gen = torch.Generator().manual_seed(1)
+    def grads():
+        for p, q in zip(ps, qs):
+            g = torch.randn(p.shape, generator=gen).to(DEV)
+            q.grad = g.clone()
+            if p.grad is None:
+                p.grad = g
+            else:
+                p.grad.copy_(g)
+    def same():
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q)
+            for k, v in twin.state[q].items():
+                if k != 'step':
+                    assert torch.equal(_bytes(opt.state[p][k]), _bytes(v)), k
+    twin.param_groups[1]['lr'] = float(torch.tensor(1e-2, dtype=torch.float32))
+    grads()
+    opt.step()
+    twin.step()
+    same()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    saved = None
+    for t in range(4):
+        if t == 2:
+            saved = copy.deepcopy(twin.state_dict()), [q.detach().clone() for q in qs]
+        grads()
+        opt.param_groups[1]['lr'].fill_(1e-2 / (t + 1))
+        twin.param_groups[1]['lr'] = float(torch.tensor(1e-2 / (t + 1), dtype=torch.float32))
+        graph.replay()
+        twin.step()
+        same()
+    sd = opt.state_dict()
+    assert all(int(s['step']) == 5 for s in sd['state'].values())
+    held = opt.param_groups[1]['lr']
+    opt.load_state_dict(saved[0])
+    twin.load_state_dict(copy.deepcopy(saved[0]))
+    opt.param_groups[1]['lr'] = held
+    with torch.no_grad():
+        for p, q, v in zip(ps, qs, saved[1]):
+            p.copy_(v)
+            q.copy_(v)
+    twin.param_groups[1]['lr'] = float(held)
+    grads()
+    graph.replay()
+    twin.step()
+    same()
+    late = torch.nn.Parameter(torch.zeros(8, device=DEV))
+    late.grad = torch.zeros(8, device=DEV)
+    for bad, says in ((AdamW([late]), 'needs capturable'), (AdamW([late], capturable=True), 'must not be a captured one')):
+        with pytest.raises(RuntimeError, match=says):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                bad.step()
+    torch.cuda.synchronize()
 
 
 # ---------------------------------------------------------------------------------------------- together
