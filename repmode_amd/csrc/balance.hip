@@ -95,12 +95,13 @@ __device__ __forceinline__ float top_of(int key) {
 
 // y_j = e^(x_j - top) of a row (y may be x), and its sum.  As 2^(x_j L - top L), L = log2(e), in one fused step: the rounding of
 // top L is the whole row's and goes out with the sum, so a probability is off by |x_j - top| 2^-24 like that of a rounded
-// difference.  Where top L leaves float32 the difference is taken first.
+// difference.  From 2^20 on, where that rounding would grow to 2^-4 and more (at last to a sum of 0 or infinity), the difference is
+// taken first.
 template <int LPR, int EPL>
 __device__ __forceinline__ float row_exp(float top, const float (&x)[EPL], float (&y)[EPL]) {
   constexpr float L = 1.44269504f;
   const float shift = top * L;
-  if (__any(fabsf(top) > 2e38f)) {
+  if (__any(fabsf(top) >= 0x1p20f)) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f((x[j] - top) * L);
   } else {
@@ -613,15 +614,15 @@ int launch_one(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   const dim3 grid((unsigned)a.blocks, (unsigned)a.groups), block(64 * BL_WAVES);
   const size_t lds = TILED ? (size_t)a.tile_rows * a.pitch * sizeof(float) : 0;
   if constexpr (TILED) {
-    static std::atomic<unsigned> allowed{0};                // per device: the tile may take more than 64 KiB
+    static std::atomic<unsigned long> allowed{0};           // per device: the tile may take more than 64 KiB
     int dev = 0;
     RM_HIP(hipGetDevice(&dev));
-    if (!(allowed.load() >> (dev & 31) & 1)) {
+    if (!(allowed.load() >> (dev & 63) & 1)) {
       const void* kernel;
       if constexpr (BWD) kernel = reinterpret_cast<const void*>(&balance_bwd_kernel<T, LPR, EPL, V, TILED>);
       else kernel = reinterpret_cast<const void*>(&balance_fwd_kernel<T, LPR, EPL, V, TILED>);
       RM_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, BL_TILE_BYTES));
-      allowed.fetch_or(1u << (dev & 31));
+      allowed.fetch_or(1ul << (dev & 63));
     }
   }
   if constexpr (BWD) hipLaunchKernelGGL((balance_bwd_kernel<T, LPR, EPL, V, TILED>), grid, block, lds, s, a);

@@ -137,6 +137,20 @@ def test_balance_loss_ties_and_infinities(experts):
         assert int(r['counts'].sum()) < 12 * 3
 
 
+@pytest.mark.parametrize('experts', [5, 24, 200, 600])
+def test_balance_loss_far_from_zero(experts):
+    """Logits of any common offset, up to the types' ends: only their differences count."""
+    gen = torch.Generator().manual_seed(experts)
+    tops = [2.0 ** e for e in (10, 18, 19.999, 20, 21, 24, 31, 40, 80, 126)] + [1e10, 1.9e38, 3.3e38]
+    x = torch.tensor([s * t for t in tops for s in (1, -1)])[:, None].expand(-1, experts).clone()
+    step = x.abs() * torch.finfo(torch.float32).eps
+    x = x - (torch.randint(0, 6, x.shape, generator=gen) * torch.maximum(step, torch.tensor(0.25))) * (torch.rand(x.shape, generator=gen) < 0.7)
+    x = x.clamp(-3.3e38, 3.3e38)
+    _check_balance(x.to(DEV), 3)
+    _check_balance(x.to(DEV).bfloat16(), 3)
+    _check_balance(x.t().contiguous().t().to(DEV), 2)
+
+
 def test_balance_loss_empty_groups():
     """Groups without a row that counts add nothing and do not count in the mean; with none at all loss and gradient are zero."""
     ops = _ops()
