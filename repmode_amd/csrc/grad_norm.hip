@@ -1,5 +1,5 @@
 // grad_norm.hip -- the 2-norm of many tensors together and the factor that clips it, without a host synchronisation:
-//     norm = sqrt(sum_i sum_e x_ie^2)          clip = min(1, max_norm / (norm + 1e-6)), NaN where the norm is not finite
+//     norm = sqrt(sum_i sum_e x_ie^2)          clip = min(1, max_norm / (norm + 1e-6)), NaN where a value is not finite
 //
 // Products and sums are float64: the square of a float32 (or bfloat16) value is exact there and cannot overflow or vanish, so
 // gradients of 1e-30 and of 1e30 count for what they are; the float64 units keep up with HBM (one conversion and one fused

@@ -1843,6 +1843,7 @@ std::tuple<Tensor, Tensor> op_grad_norm(const TensorList& tensors, double max_no
   for (size_t i = 0; i < n; ++i) {
     const Tensor& t = tensors.get(i);
     require_hip(t, "grad_norm: tensor");
+    TORCH_CHECK(t.layout() == at::kStrided, "grad_norm: tensor ", i, " is not strided");
     (void)dtype_code(t.scalar_type());
     TORCH_CHECK(t.device() == dev, "grad_norm: tensor ", i, " is on ", t.device(), ", tensor 0 on ", dev);
   }
@@ -1919,7 +1920,8 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
     require_hip(p, "adamw_step: a parameter");
     const bool eight = mt == at::kFloat8_e4m3fn;
     kind[i] = (char)((dtype_code(dt) == REPMODE_BF16 ? 1 : 0) | (eight ? 2 : 0));
-    TORCH_CHECK(p.device() == dev && p.is_non_overlapping_and_dense(), "adamw_step: parameter ", i, ": dense tensors on one device");
+    TORCH_CHECK(p.layout() == at::kStrided && p.device() == dev && p.is_non_overlapping_and_dense(), "adamw_step: parameter ", i,
+                ": dense tensors on one device");
     TORCH_CHECK(g.layout() == at::kStrided && g.device() == dev && g.scalar_type() == dt && g.sizes() == p.sizes(),
                 "adamw_step: gradient ", i, ": the parameter's type, shape and device");
     TORCH_CHECK((eight || mt == at::kFloat) && v.scalar_type() == (eight ? at::kFloat8_e5m2 : at::kFloat),
@@ -2054,6 +2056,7 @@ bool op_graph_alive(const std::vector<Tensor>& leaves) {
 
 std::tuple<Tensor, Tensor, Tensor> op_balance_loss(const Tensor& logits, const OptTensor& mask, int64_t top_k, double coef) {
   require_hip(logits, "balance_loss: logits");
+  TORCH_CHECK(logits.layout() == at::kStrided, "balance_loss: strided logits");
   (void)dtype_code(logits.scalar_type());
   TORCH_CHECK(logits.dim() == 2 || logits.dim() == 3, "balance_loss: logits are [rows, experts] or [groups, rows, experts], got ", logits.sizes());
   const int64_t groups = logits.dim() == 3 ? logits.size(0) : 1, rows = logits.size(-2), experts = logits.size(-1);

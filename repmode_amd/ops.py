@@ -394,7 +394,7 @@ ADAMW_BLOCK = 256       # elements that share a power of two in the 8-bit moment
 def grad_norm(tensors, max_norm=None):
     """``(norm, clip)``: the 2-norm of all ``tensors`` together (float32 or bfloat16, any strides; sums in float64, in a fixed
     order) and the factor ``min(1, max_norm / (norm + 1e-6))`` that clips them, both float32 scalars on the device -- no
-    synchronisation, nothing is scaled here.  ``clip`` is NaN where the norm is not finite (``adamw_step`` then leaves the
+    synchronisation, nothing is scaled here.  ``clip`` is NaN where a value is not finite (``adamw_step`` then leaves the
     step out); without ``max_norm`` it is 1.  No autograd."""
     return list_ops().grad_norm(list(tensors), float('inf') if max_norm is None else float(max_norm))
 

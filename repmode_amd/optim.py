@@ -138,7 +138,7 @@ class AdamW(torch.optim.Optimizer):
     and the moments in float32 or in 8 bits (csrc/adamw.hip, csrc/grad_norm.hip).  float32 and bfloat16 parameters.
 
     ``max_norm``: the gradients of all groups together are scaled by ``min(1, max_norm / (norm + 1e-6))`` on their way into the
-    update (``.grad`` itself stays as it is; ``last_norm`` is the norm, a device scalar).  Where the norm is not finite the step
+    update (``.grad`` itself stays as it is; ``last_norm`` is the norm, a device scalar).  Where a gradient is not finite the step
     changes no parameter and no moment.
     ``state_bits``: 32, or 8 -- e4m3 / e5m2 values with a power of two for each 256 elements, rounded stochastically: 2 bytes a
     parameter instead of 8.  Tensors of fewer than ``min_8bit_numel`` elements (biases, norms) keep float32 moments.  Both may be
@@ -230,10 +230,10 @@ class AdamW(torch.optim.Optimizer):
 
     def _count_on_device(self, gi, steps, device):
         """The group's step count on the device; ``steps``: its parameters' host counters, which go on as well."""
+        t0 = {int(s) for s in steps}
+        if len(t0) != 1:                       # (also where a parameter has its first gradient after the others)
+            raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): the parameters of a group must have seen the same number of steps')
         if gi not in self._step_dev:
-            t0 = {int(s) for s in steps}
-            if len(t0) != 1:
-                raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): the parameters of a group must have seen the same number of steps')
             if _capturing():
                 raise RuntimeError('repmode_amd.optim.AdamW(capturable=True): run one step launch by launch before capturing')
             self._step_dev[gi] = torch.full((1,), t0.pop(), dtype=torch.int64, device=device)

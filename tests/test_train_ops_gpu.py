@@ -796,6 +796,30 @@ def test_adamw_optimizer_in_a_graph():
     torch.cuda.synchronize()
 
 
+def test_adamw_on_device_counts_are_a_groups():
+    """capturable: a parameter whose first gradient comes after the others' would be corrected by their step count: refused."""
+    from repmode_amd.optim import AdamW
+    _ops()
+    ps = [torch.nn.Parameter(torch.ones(8, device=DEV)) for _ in range(2)]
+    opt = AdamW(ps, capturable=True)
+    ps[0].grad = torch.ones(8, device=DEV)
+    opt.step()
+    ps[1].grad = torch.ones(8, device=DEV)
+    with pytest.raises(RuntimeError, match='same number of steps'):
+        opt.step()
+    assert torch.equal(ps[1].detach(), torch.ones(8, device=DEV))
+
+
+def test_operators_take_strided_tensors():
+    ops = _ops()
+    t = torch.zeros(4, 4, device=DEV)
+    s = torch.sparse_coo_tensor(torch.zeros(2, 1, dtype=torch.long, device=DEV), torch.ones(1, device=DEV), (4, 4))
+    for call in (lambda: ops.grad_norm([t, s]), lambda: ops.balance_loss(s, 1), lambda: ops.adamw_step([s], [t], [t.clone()], [t.clone()], 1),
+                 lambda: ops.adamw_step([t], [s], [t.clone()], [t.clone()], 1)):
+        with pytest.raises(RuntimeError, match='strided|dense|gradient 0'):
+            call()
+
+
 # ---------------------------------------------------------------------------------------------- together
 
 def _stock_twin(params, **kw):
