@@ -534,7 +534,7 @@ int repmode_grad_norm_finish(const double* partial, long n, double max_norm, flo
 
 /* ---- load-balance loss of a router or of a mixture's gates, per-expert counts, gradient (csrc/balance.hip) ----
  * x: logits [groups][rows][experts] with element strides sg, sn, se, float32 or bfloat16; mask: bytes [groups][rows] with strides
- * mg, mn, 0 = the row does not count (it is not read), or NULL.  A row of -inf alone does not count either.  With p = softmax(x),
+ * mg, mn, 0 = the row does not count (whatever it holds), or NULL.  A row of -inf alone does not count either.  With p = softmax(x),
  * the top_k largest of each row chosen (ties: the lowest index; never a -inf), f_ge the share of group g's choices that are e and
  * P_ge the mean of its p_e:  loss = coef * experts * mean over the groups that have rows of sum_e f_ge P_ge.
  *   counts int64, prob float [groups][experts]: choices, mean probabilities.  weight: float [groups * experts + 1], for the

@@ -10,7 +10,7 @@
 //
 // A row's E values live in the registers of LPR lanes, 8 (E > 512: 16) a lane, so a row is read once and softmax, choice and
 // the lane's share of the column sums (probabilities in float32, counts as integers) need no memory.
-//   The choice needs no order, only the k-th largest value: each lane sorts its values once (a network), then top_k rounds take the
+//   The choice needs no order, only the k-th largest value: each lane sorts its values once (a network of 2- and 3-sorters), then top_k rounds take the
 // row's largest head and move the list of the lane that holds it up by one; what is at least the last round's value is chosen.
 // The first round's value is the softmax's maximum.  All of it on integers that are ordered as the values are; bfloat16
 // values carry their index in the lower half, so no two are equal; float32 rows where more than top_k values
@@ -18,11 +18,12 @@
 //   A workgroup walks many rows and writes one partial per expert; one launch adds the partials of a group's columns in a fixed
 // order in float64, one more makes the loss of them; where one workgroup has seen all rows it does both itself.  No float atomics: a
 // run repeats itself bit by bit.  The backward pass reads the logits again and needs nothing of a row but its logits.
-// What bounds it: the backward pass HBM (one read, one write: 262144 x 256 float32 logits 84 us, 6.4 TB/s), the forward pass the
-// instructions of exponential and choice (the same logits 67 us for the top 1, 83 for the top 8 and 9 for the columns, where a read
-// takes 40).
+// What bounds it: the backward pass HBM (one read, one write: 262144 x 256 float32 logits 82 us, 6.5 TB/s), the forward pass the
+// instructions of exponential and choice (the same logits 69 us for the top 8 and 5 for the columns, where a read takes 40; the top 1
+// some 20 us less).
 #include "common.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 
@@ -31,6 +32,7 @@ namespace {
 constexpr int BL_WAVES = 8;
 constexpr int BL_MAX_E = REPMODE_BALANCE_MAX_EXPERTS;
 constexpr int BL_TILE_BYTES = 72 << 10;  // of a tile: two workgroups share a CU's LDS
+constexpr int BL_JOIN = BL_WAVES * (sizeof(float) + sizeof(int));      // bytes a column of a row takes where a workgroup's waves are joined
 constexpr int BL_FINISH = 256;           // threads of the finish
 constexpr int BL_COLUMNS = 4;            // columns of a workgroup of it; the other threads share the partials
 constexpr int BL_BLOCKS = 512;           // most workgroups of a pass: two to a CU, which registers leave room for
@@ -108,28 +110,57 @@ __device__ __forceinline__ float row_exp(float top, const float (&x)[EPL], float
 #pragma unroll
     for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(x[j], L, -shift));
   }
-  float sum = 0.f;
+  float sum = y[0];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) sum += y[j];
+  for (int j = 1; j < EPL; ++j) sum += y[j];
   return row_sum<LPR>(sum);
 }
 
-// descending, by Batcher's odd-even merges
+__device__ __forceinline__ void sort2(int& a, int& b) {
+  const int x = a, y = b;
+  a = max(x, y);
+  b = min(x, y);
+}
+// One instruction for each of the three.  (Spelled with minima and maxima the median would share their first steps with the others, and
+// none of the three be one instruction.  No lane shift reads its result: the rounds below shift what a selection or a maximum made.)
+__device__ __forceinline__ void sort3(int& a, int& b, int& c) {
+  const int x = a, y = b, z = c;
+  a = max(max(x, y), z);
+  asm("v_med3_i32 %0, %1, %2, %3" : "=v"(b) : "v"(x), "v"(y), "v"(z));
+  c = min(min(x, y), z);
+}
+// Eight values, descending: as the columns (0 1 2) (3 4 5) (6 7) of a square whose columns and then rows are sorted (which keeps the
+// columns so).  0 is the largest then.  Of its diagonal 2 4 6, sorted, two at least lie below both of 1 and 3 (4, and one's neighbour), so
+// only the largest may lie above the smaller of those; 5 and 7 likewise.  27 instructions, where pairs alone take 38.
+__device__ __forceinline__ void sort8(int* s) {
+  sort3(s[0], s[1], s[2]);
+  sort3(s[3], s[4], s[5]);
+  sort2(s[6], s[7]);
+  sort3(s[0], s[3], s[6]);
+  sort3(s[1], s[4], s[7]);
+  sort2(s[2], s[5]);
+  sort3(s[2], s[4], s[6]);
+  sort2(s[1], s[3]);
+  sort2(s[5], s[7]);
+  sort2(s[3], s[2]);
+  sort2(s[6], s[5]);
+  const int third = s[3], fourth = s[2], fifth = s[4], sixth = s[6], seventh = s[5];
+  s[2] = third; s[3] = fourth; s[4] = fifth; s[5] = sixth; s[6] = seventh;
+}
+// descending: eights, then Batcher's odd-even merges
 template <int N>
 __device__ __forceinline__ void sort_descending(int (&s)[N]) {
 #pragma unroll
-  for (int p = 1; p < N; p *= 2)
+  for (int j = 0; j < N; j += 8) sort8(s + j);
+#pragma unroll
+  for (int p = 8; p < N; p *= 2)
 #pragma unroll
     for (int k = p; k >= 1; k /= 2)
 #pragma unroll
       for (int j = k % p; j + k < N; j += 2 * k)
 #pragma unroll
         for (int i = 0; i < k; ++i)
-          if ((i + j) / (2 * p) == (i + j + k) / (2 * p) && i + j + k < N) {
-            const int a = s[i + j], b = s[i + j + k];
-            s[i + j] = max(a, b);
-            s[i + j + k] = min(a, b);
-          }
+          if ((i + j) / (2 * p) == (i + j + k) / (2 * p) && i + j + k < N) sort2(s[i + j], s[i + j + k]);
 }
 
 // the lane whose head is t moves its list up by one, as far as N values of it are looked at afterwards
@@ -161,7 +192,7 @@ __device__ __forceinline__ int row_kth(int (&s)[EPL], int top, int top_k) {
   if constexpr (LPR == 1) {
 #pragma unroll
     for (int j = 1; j < EPL; ++j) t = j < top_k ? +s[j] : t;
-  } else if (top_k <= EPL) {
+  } else if (__builtin_expect(top_k <= EPL, 1)) {
     t = rounds_from<LPR, 1>(s, t, top_k);
   } else {
     for (int k = 1; k < top_k; ++k) {
@@ -176,30 +207,44 @@ __device__ __forceinline__ int row_kth(int (&s)[EPL], int top, int top_k) {
 template <int LPR, int V>
 __device__ __forceinline__ int expert_of(int j, int sub) { return (j / V) * (LPR * V) + sub * V + j % V; }
 
-// a lane's values of a row; -inf where there is none, and everywhere in a row that does not count
+// A lane's values of a row as they are in memory.  Every load is made, in a straight line -- past the row's last value that again -- since
+// behind loads that may or may not have been made there is one wait for all that are under way, and behind each of them one where
+// its value is converted.
+template <typename T, int EPL, int V>
+struct RawRow {
+  std::conditional_t<V == 1, T, u32x4> w[EPL / V];
+};
 template <typename T, int LPR, int EPL, int V>
-__device__ __forceinline__ void load_row(const BalanceArgs& a, const T* row, bool on, int sub, float (&x)[EPL]) {
+__device__ __forceinline__ void fetch_row(const BalanceArgs& a, const T* row, int sub, RawRow<T, EPL, V>& r) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) x[j] = -INFINITY;
+  for (int q = 0; q < EPL / V; ++q) {
+    const int e = min(expert_of<LPR, V>(q * V, sub), a.experts - V);          // (V divides the experts)
+    if constexpr (V == 1) r.w[q] = row[(long)e * a.se];
+    else r.w[q] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + e));
+  }
+}
+// as floats; -inf where there is none, and everywhere in a row that does not count
+template <typename T, int LPR, int EPL, int V>
+__device__ __forceinline__ void row_values(const BalanceArgs& a, const RawRow<T, EPL, V>& r, bool on, int sub, float (&x)[EPL]) {
 #pragma unroll
-  for (int j = 0; j < EPL; j += V) {
-    const int e = expert_of<LPR, V>(j, sub);
-    if (!on || e >= a.experts) continue;                    // (V divides the experts)
+  for (int q = 0; q < EPL / V; ++q) {
     if constexpr (V == 1) {
-      x[j] = to_f32<T>(row[(long)e * a.se]);
+      x[q] = to_f32<T>(r.w[q]);
     } else {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(row + e);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (sizeof(T) == 4) {
-          x[j + k] = __uint_as_float(w[k]);
+          x[q * V + k] = __uint_as_float(r.w[q][k]);
         } else {
-          x[j + 2 * k] = __uint_as_float(w[k] << 16);
-          x[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+          x[q * V + 2 * k] = __uint_as_float(r.w[q][k] << 16);
+          x[q * V + 2 * k + 1] = __uint_as_float(r.w[q][k] & 0xffff0000u);
         }
       }
     }
   }
+  if (a.experts == LPR * EPL && __all(on)) return;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) x[j] = on && expert_of<LPR, V>(j, sub) < a.experts ? x[j] : -INFINITY;
 }
 
 // Logits whose rows, not experts, are neighbours in memory: a tile of rows is read along them into LDS, [row][expert] with an odd
@@ -208,16 +253,25 @@ template <typename T>
 __device__ __forceinline__ void load_tile(const BalanceArgs& a, const T* x0, const uint8_t* mask, long n0, float* tile) {
   constexpr int AHEAD = 8;
   const int r = threadIdx.x % a.tile_rows, e0 = threadIdx.x / a.tile_rows, step = 64 * BL_WAVES / a.tile_rows;
-  const long n = n0 + r;
-  const bool on = n < a.rows && (!mask || mask[n * a.mn]);
+  const long n = min(n0 + r, a.rows - 1);
+  const bool on = n == n0 + r && (!mask || mask[n * a.mn]);
   const T* x = x0 + n * a.sn;
-  for (int e = e0; e < a.experts; e += AHEAD * step) {
-    float v[AHEAD];
+  int e = e0;
+  for (; e - e0 + AHEAD * step <= a.experts; e += AHEAD * step) {
+    const T* from = x + (long)e * a.se;
+    T v[AHEAD];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) v[u] = on && e + u * step < a.experts ? to_f32<T>(x[(long)(e + u * step) * a.se]) : -INFINITY;
+    for (int u = 0; u < AHEAD; ++u) v[u] = from[(long)(u * step) * a.se];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) tile[r * a.pitch + e + u * step] = on ? to_f32<T>(v[u]) : -INFINITY;
+  }
+  if (e - e0 < a.experts) {
+    T v[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) v[u] = x[(long)min(e + u * step, a.experts - 1) * a.se];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      if (e + u * step < a.experts) tile[r * a.pitch + e + u * step] = v[u];
+      if (e + u * step < a.experts) tile[r * a.pitch + e + u * step] = on ? to_f32<T>(v[u]) : -INFINITY;
   }
 }
 template <int LPR, int EPL>
@@ -336,7 +390,7 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
     const float inv = counts ? __builtin_amdgcn_rcpf(sum) : 0.f;         // (1 ulp; 1 <= sum <= experts)
 #pragma unroll
     for (int j = 0; j < EPL; ++j) psum[j] = fmaf(x[j], inv, psum[j]);
-    valid += counts && sub == 0;
+    valid += __popcll(__ballot(counts));                    // (the wave's, LPR for each row)
     choose<T, LPR, EPL, V>(key, row_kth<LPR>(s, top, a.top_k), sub, a.top_k, cnt);
   };
   if constexpr (TILED) {
@@ -352,32 +406,48 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
       __syncthreads();
     }
   } else {
-    const long step = (long)a.blocks * BL_WAVES * RPW;
-    float x[EPL], next[EPL];
-    long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW;
-    const T* row = x0 + (n0 + slot) * a.sn;
-    long masked = (n0 + slot) * a.mn;
-    auto fetch = [&](float (&to)[EPL], long n) {
-      load_row<T, LPR, EPL, V>(a, row, n < a.rows && (!mask || mask[masked]), sub, to);
-      row += step * a.sn;
-      masked += step * a.mn;
+    // Rows are fetched while those before them are worked on, into two sets of registers that take turns; behind the last rows the last
+    // again.
+    const unsigned step = a.blocks * BL_WAVES * RPW, end = (unsigned)a.rows;          // (rows < 2^31, step <= 2^18)
+    unsigned n0 = (blockIdx.x * BL_WAVES + wave) * RPW;
+    const long slot_at = slot * a.sn;
+    const T* rows = x0 + (long)n0 * a.sn;
+    auto walk = [&](auto has_mask) {
+      constexpr bool MASKED = decltype(has_mask)::value;
+      struct Rows {
+        RawRow<T, EPL, V> row;
+        uint8_t on;
+      };
+      auto fetch = [&](Rows& to, unsigned n, const T* from) {
+        long at = slot_at;
+        unsigned in = slot;
+        if (n + RPW > end) {
+          in = min(in, end - 1 - n);
+          at = in * a.sn;
+        }
+        fetch_row<T, LPR, EPL, V>(a, from + at, sub, to.row);
+        if constexpr (MASKED) to.on = mask[(long)(n + in) * a.mn];
+      };
+      auto turn_of = [&](Rows& now, Rows& then) {             // whether there are more
+        const bool more = n0 + step < end;
+        const unsigned n = n0;
+        n0 += more ? step : 0;
+        rows += more ? step * a.sn : 0;
+        fetch(then, n0, rows);
+        float x[EPL];
+        bool on = n + slot < end;
+        if constexpr (MASKED) on = on && now.on;
+        row_values<T, LPR, EPL, V>(a, now.row, on, sub, x);
+        work(x);
+        return more;
+      };
+      Rows even, odd;
+      fetch(even, n0, rows);
+      while (turn_of(even, odd) && turn_of(odd, even)) {}
     };
-    // A row is fetched while the one before it is worked on.  Two sets of registers take turns; with 16 values a lane the second copy of
-    // the work costs more registers than it saves moves (1024 experts: 97 us, with moves 88; 256: 68 and 76).
-    if (n0 < a.rows) fetch(x, n0 + slot);
-    while (n0 < a.rows) {
-      n0 += step;
-      if (n0 < a.rows) fetch(next, n0 + slot);
-      work(x);
-      if (n0 >= a.rows) break;
-      if constexpr (EPL > 8) {
-#pragma unroll
-        for (int j = 0; j < EPL; ++j) x[j] = next[j];
-      } else {
-        n0 += step;
-        if (n0 < a.rows) fetch(x, n0 + slot);
-        work(next);
-      }
+    if (n0 < end) {
+      if (mask) walk(std::true_type{});
+      else walk(std::false_type{});
     }
   }
   // the wave's rows, then the workgroup's waves
@@ -389,11 +459,12 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
       cnt[j] += __shfl_xor(cnt[j], off, 64);
     }
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) valid += __shfl_xor(valid, off, 64);
-  __shared__ float sp[BL_WAVES][LPR * EPL];
-  __shared__ int sc[BL_WAVES][LPR * EPL], sv[BL_WAVES];
+  __shared__ int sv[BL_WAVES];
   __shared__ double st[BL_WAVES];
+  __shared__ __align__(16) char own[TILED ? 1 : BL_JOIN * LPR * EPL];
+  extern __shared__ float tile[];                           // (of a tiled pass, whose rows are done with)
+  float(*sp)[LPR * EPL] = reinterpret_cast<float(*)[LPR * EPL]>(TILED ? reinterpret_cast<char*>(tile) : own);
+  int(*sc)[LPR * EPL] = reinterpret_cast<int(*)[LPR * EPL]>(sp + BL_WAVES);
   if (slot == 0) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
@@ -401,7 +472,7 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
       sc[wave][expert_of<LPR, V>(j, sub)] = cnt[j];
     }
   }
-  if (lane == 0) sv[wave] = valid;
+  if (lane == 0) sv[wave] = valid / LPR;
   __syncthreads();
   int rows = 0;
 #pragma unroll
@@ -438,37 +509,47 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_fwd_kernel(BalanceArgs 
 // BL_COLUMNS columns of a group: counts, mean probabilities, weights (but for 1 / G') and this part of sum_e f_e P_e
 __global__ __launch_bounds__(BL_FINISH) void balance_columns_kernel(FinishArgs a) {
   constexpr int SHARES = BL_FINISH / BL_COLUMNS, AHEAD = 8;
+  static_assert(64 % BL_COLUMNS == 0, "a wave holds whole shares");
   const int g = blockIdx.y, col = threadIdx.x % BL_COLUMNS, share = threadIdx.x / BL_COLUMNS, e = blockIdx.x * BL_COLUMNS + col;
-  __shared__ double sp[SHARES][BL_COLUMNS];
-  __shared__ long sc[SHARES][BL_COLUMNS], sn[BL_FINISH / 64];
+  __shared__ double sp[BL_FINISH / 64][BL_COLUMNS];
+  __shared__ long sc[BL_FINISH / 64][BL_COLUMNS], sn[BL_FINISH / 64];
   double p = 0;
   long c = 0, n = 0;
-  if (e < a.experts) {
-    const long at = (long)g * a.blocks * a.experts + e;
-    for (int b0 = share; b0 < a.blocks; b0 += AHEAD * SHARES) {
-      float v[AHEAD];
-      int w[AHEAD];
+  const long at = (long)g * a.blocks * a.experts + min(e, a.experts - 1);
+  for (int b0 = 0; b0 < a.blocks; b0 += AHEAD * SHARES) {      // (every load is made: behind the last partial the last again)
+    float v[AHEAD];
+    int w[AHEAD];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int b = b0 + u * SHARES;
-        v[u] = b < a.blocks ? a.psum[at + (long)b * a.experts] : 0.f;
-        w[u] = b < a.blocks ? a.count[at + (long)b * a.experts] : 0;
-      }
+    for (int u = 0; u < AHEAD; ++u) {
+      const long b = at + (long)min(b0 + u * SHARES + share, a.blocks - 1) * a.experts;
+      v[u] = a.psum[b];
+      w[u] = a.count[b];
+    }
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) { p += v[u]; c += w[u]; }
+    for (int u = 0; u < AHEAD; ++u) {
+      const bool in = b0 + u * SHARES + share < a.blocks;
+      p += in ? v[u] : 0.f;
+      c += in ? w[u] : 0;
     }
   }
   for (int b = threadIdx.x; b < a.blocks; b += BL_FINISH) n += a.valid[(long)g * a.blocks + b];
 #pragma unroll
+  for (int off = 32; off >= BL_COLUMNS; off >>= 1) {          // the wave's shares of a column
+    p += __shfl_xor(p, off, 64);
+    c += __shfl_xor(c, off, 64);
+  }
+#pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-  sp[share][col] = p;
-  sc[share][col] = c;
+  if ((threadIdx.x & 63) < BL_COLUMNS) {
+    sp[threadIdx.x >> 6][col] = p;
+    sc[threadIdx.x >> 6][col] = c;
+  }
   if ((threadIdx.x & 63) == 0) sn[threadIdx.x >> 6] = n;
   __syncthreads();
   if (threadIdx.x >= 64) return;
   p = 0; c = 0; n = 0;
-  for (int s = 0; s < SHARES; ++s) { p += sp[s][col]; c += sc[s][col]; }
-  for (int w = 0; w < BL_FINISH / 64; ++w) n += sn[w];
+#pragma unroll
+  for (int w = 0; w < BL_FINISH / 64; ++w) { p += sp[w][col]; c += sc[w][col]; n += sn[w]; }
   const double term = wave_sum(share == 0 && e < a.experts ? finish_expert(a, g, e, p, c, n) : 0.0);
   if (threadIdx.x == 0) {
     a.term[(long)g * gridDim.x + blockIdx.x] = term;
@@ -502,10 +583,9 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs 
   const float scale = *a.up * a.weight[(long)a.groups * a.experts];
   float w[EPL];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    const int e = expert_of<LPR, V>(j, sub);
-    w[j] = e < a.experts ? scale * a.weight[(long)g * a.experts + e] : 0.f;
-  }
+  for (int j = 0; j < EPL; ++j) w[j] = a.weight[(long)g * a.experts + min(expert_of<LPR, V>(j, sub), a.experts - 1)];
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) w[j] = expert_of<LPR, V>(j, sub) < a.experts ? scale * w[j] : 0.f;
   auto work = [&](float (&x)[EPL]) {                        // logits in, gradients out
     int top = turn(__float_as_int(x[0]));
 #pragma unroll
@@ -555,10 +635,12 @@ __global__ __launch_bounds__(64 * BL_WAVES) void balance_bwd_kernel(BalanceArgs 
   }
   const long step = (long)a.blocks * BL_WAVES * RPW;
   for (long n0 = ((long)blockIdx.x * BL_WAVES + wave) * RPW; n0 < a.rows; n0 += step) {
-    const long n = n0 + slot;
-    const bool in = n < a.rows, on = in && (!mask || mask[n * a.mn]);
+    const long n = min(n0 + slot, a.rows - 1);
+    const bool in = n == n0 + slot;
+    RawRow<T, EPL, V> raw;
     float x[EPL];
-    load_row<T, LPR, EPL, V>(a, x0 + n * a.sn, on, sub, x);
+    fetch_row<T, LPR, EPL, V>(a, x0 + n * a.sn, sub, raw);
+    row_values<T, LPR, EPL, V>(a, raw, in && (!mask || mask[n * a.mn]), sub, x);
     work(x);
     if (!in) continue;
     T* row = d0 + n * a.dn;
@@ -612,7 +694,7 @@ int blocks_for(long groups, long rows, int experts) {
 template <typename T, bool BWD, int LPR, int EPL, int V, bool TILED>
 int launch_one(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   const dim3 grid((unsigned)a.blocks, (unsigned)a.groups), block(64 * BL_WAVES);
-  const size_t lds = TILED ? (size_t)a.tile_rows * a.pitch * sizeof(float) : 0;
+  const size_t lds = TILED ? std::max((size_t)a.tile_rows * a.pitch * sizeof(float), (size_t)(BWD ? 0 : BL_JOIN * LPR * EPL)) : 0;
   if constexpr (TILED) {
     static std::atomic<unsigned long> allowed{0};           // per device: the tile may take more than 64 KiB
     int dev = 0;
@@ -636,7 +718,7 @@ int launch(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
   switch (lanes_per_row(a.experts)) {
     case 1: return launch_one<T, BWD, 1, 8, V, false>(a, f, s);
     case 2: return launch_one<T, BWD, 2, 8, V, false>(a, f, s);
-    case 4: return launch_one<T, BWD, 4, 8, V, false>(a, f, s);
+    case 4: return launch_one<T, BWD, 4, 8, V, TILED && BWD>(a, f, s);
     case 8: return launch_one<T, BWD, 8, 8, V, TILED>(a, f, s);
     case 16: return launch_one<T, BWD, 16, 8, V, TILED>(a, f, s);
     case 32: return launch_one<T, BWD, 32, 8, V, TILED>(a, f, s);
@@ -646,11 +728,10 @@ int launch(const BalanceArgs& a, const FinishArgs& f, hipStream_t s) {
 
 // A pass with the form its strides ask for:
 //   16-byte pieces where every row has them: consecutive experts, rows that start at 16 bytes and hold whole pieces;
-//   tiles where the rows are neighbours and a row takes 8 lanes or more, so that a wave's loads along the experts would take 32 bytes
-// or less of a cache line (2^26 float32 logits, 32 / 64 / 128 / 512 experts, tiles and without: forward 103 / 104 / 101 / 145 us and
-// 76 / 103 / 194 / 556, backward 166 / 157 / 152 / 163 and 198 / 278 / 473 / 1056; bfloat16 backward 165 / 179 / 176 / 187 and 132 /
-// 190 / 295 / 1485).  Not for the forward pass of bfloat16, whose tiles' 2-byte loads cost what they save (149 / 147 / 260 and 123 /
-// 143 / 230);
+//   tiles where the rows are neighbours and a row takes so many lanes that a wave's loads along the experts would leave most of a cache
+// line -- forward from 8 (2^26 float32 logits, 32 / 64 / 128 / 512 experts, tiles and without, top 1: 92 / 86 / 84 / 87 us and 86 / 135 /
+// 235 / 446; bfloat16 73 / 71 / 70 / 78 and 59 / 103 / 148 / 515), backward, which would leave the lines it writes too, from 4 (16 / 24 /
+// 64 / 512 experts: 154 / 153 / 137 / 146 and 142 / 247 / 255 / 997; bfloat16 127 / 133 / 110 / 131 and 120 / 180 / 236 / 1132);
 //   else element by element.
 template <bool BWD>
 int dispatch(BalanceArgs a, FinishArgs* finish, int dtype, hipStream_t s) {
@@ -662,7 +743,7 @@ int dispatch(BalanceArgs a, FinishArgs* finish, int dtype, hipStream_t s) {
   };
   if (a.experts % per == 0 && whole(a.x, a.sg, a.sn, a.se) && (!BWD || whole(a.dx, a.dg, a.dn, a.de)))
     return dtype == REPMODE_F32 ? launch<float, BWD, 4, false>(a, f, s) : launch<bf16_t, BWD, 8, false>(a, f, s);
-  if (a.se != 1 && a.sn == 1 && lanes_per_row(a.experts) >= 8 && (BWD || dtype == REPMODE_F32)) {
+  if (a.se != 1 && a.sn == 1 && lanes_per_row(a.experts) >= (BWD ? 4 : 8)) {
     a.pitch = a.experts | 1;
     a.tile_rows = 64 * BL_WAVES;
     while ((size_t)a.tile_rows * a.pitch * sizeof(float) > BL_TILE_BYTES) a.tile_rows /= 2;
@@ -670,18 +751,15 @@ int dispatch(BalanceArgs a, FinishArgs* finish, int dtype, hipStream_t s) {
     // (a tile is rows for at least two rounds of the workgroup, so there are never more workgroups than the plan has)
     if (tiles < a.blocks) a.blocks = (int)(tiles < 1 ? 1 : tiles);
     if (finish) finish->blocks = f.blocks = a.blocks;
-    if constexpr (BWD) {
-      if (dtype == REPMODE_BF16) return launch<bf16_t, BWD, 1, true>(a, f, s);
-    }
-    return launch<float, BWD, 1, true>(a, f, s);
+    return dtype == REPMODE_F32 ? launch<float, BWD, 1, true>(a, f, s) : launch<bf16_t, BWD, 1, true>(a, f, s);
   }
   return dtype == REPMODE_F32 ? launch<float, BWD, 1, false>(a, f, s) : launch<bf16_t, BWD, 1, false>(a, f, s);
 }
 
 int check_shape(const char* who, const void* x, int dtype, long groups, long rows, int experts) {
   RM_REQUIRE(dtype == REPMODE_F32 || dtype == REPMODE_BF16, "%s: bad dtype %d", who, dtype);
-  RM_REQUIRE(groups > 0 && groups <= 65535 && rows >= 0 && experts > 0 && experts <= BL_MAX_E,
-             "%s: 1..65535 groups, 1..%d experts; got %ld groups of %ld rows over %d experts", who, BL_MAX_E, groups, rows, experts);
+  RM_REQUIRE(groups > 0 && groups <= 65535 && rows >= 0 && rows < (1L << 31) && experts > 0 && experts <= BL_MAX_E,
+             "%s: 1..65535 groups of less than 2^31 rows, 1..%d experts; got %ld groups of %ld rows over %d experts", who, BL_MAX_E, groups, rows, experts);
   RM_REQUIRE(x || rows == 0, "%s: null pointer", who);
   return REPMODE_OK;
 }

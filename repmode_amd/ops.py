@@ -440,7 +440,7 @@ def balance_loss(logits, top_k, mask=None, coef=1.0):
 
         loss = coef * experts * mean over the groups that have rows of sum_e f_e P_e        (coef, where all are used alike)
 
-    ``mask``: bool, False = the row does not count and is not read (padding).  ``counts`` (int64) and ``prob`` (float32), [experts]
+    ``mask``: bool, False = the row does not count, whatever it holds (padding).  ``counts`` (int64) and ``prob`` (float32), [experts]
     or [groups, experts]: the choices of each expert and its mean probability.  The loss's gradient reaches the logits through p;
     counts and prob carry none.  A NaN in a row that counts makes the loss NaN."""
     return torch_ops().balance_loss(logits, mask, int(top_k), float(coef))
