@@ -80,7 +80,14 @@ static_assert(sizeof(AdamWArgs) <= 4096, "launch arguments");
 // (4 / 32 / 128 M float32 parameters, float32 moments: 24.6 / 162 / 640 us, through the caches 32.0 / 184 / 706; right after the norm
 // of the same gradients 20.7 / 144 / 603 and 25.0 / 160 / 663.  Only a list of tens of MB that is updated again and again with nothing
 // in between would gain by the caches: 28.3 and 26.1 at 4 M.)
+// AW_PART: element by element, `left` of them in the tensor; every load is made -- past the end the last element again, left > 0 or not --
+// so that one wait does for all of a lane's.
 enum { AW_PART = 0, AW_WHOLE = 1, AW_SOME = 2 };
+template <typename E>
+__device__ __forceinline__ void load_part(const E* p, int left, E (&e)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) e[k] = p[min(k, left - 1)];
+}
 template <typename V>
 __device__ __forceinline__ V fetch(const V* p) { return __builtin_nontemporal_load(p); }
 template <typename V>
@@ -88,11 +95,9 @@ __device__ __forceinline__ void put(V* p, const V& x) { __builtin_nontemporal_st
 template <int HOW>
 __device__ __forceinline__ f32x4 load4(const float* p, int left) {
   if constexpr (HOW != AW_PART) return fetch(reinterpret_cast<const f32x4*>(p));
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (k < left) r[k] = p[k];
-  return r;
+  float e[4];
+  load_part(p, left, e);
+  return f32x4{e[0], e[1], e[2], e[3]};
 }
 template <int HOW>
 __device__ __forceinline__ f32x4 load4(const bf16_t* p, int left) {
@@ -100,20 +105,16 @@ __device__ __forceinline__ f32x4 load4(const bf16_t* p, int left) {
     const u32x2 w = fetch(reinterpret_cast<const u32x2*>(p));
     return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
   }
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (k < left) r[k] = bf16_to_f32(p[k]);
-  return r;
+  bf16_t e[4];
+  load_part(p, left, e);
+  return f32x4{bf16_to_f32(e[0]), bf16_to_f32(e[1]), bf16_to_f32(e[2]), bf16_to_f32(e[3])};
 }
 template <int HOW>
 __device__ __forceinline__ uint32_t load4(const uint8_t* p, int left) {
   if constexpr (HOW != AW_PART) return fetch(reinterpret_cast<const uint32_t*>(p));
-  uint32_t r = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (k < left) r |= (uint32_t)p[k] << (8 * k);
-  return r;
+  uint8_t e[4];
+  load_part(p, left, e);
+  return (uint32_t)e[0] | (uint32_t)e[1] << 8 | (uint32_t)e[2] << 16 | (uint32_t)e[3] << 24;
 }
 template <int HOW>
 __device__ __forceinline__ void store4(float* p, const f32x4& x, int left) {

@@ -84,7 +84,15 @@ __global__ __launch_bounds__(GN_THREADS) void grad_norm_kernel(NormArgs a, doubl
       }
     rest += (long)pieces * VEC;
   }
-  for (long o = rest + threadIdx.x; o < end; o += GN_THREADS) add(to_f32<T>(x[o]));
+  constexpr int AHEAD = 8;
+  for (long o = rest + threadIdx.x; o < end; o += AHEAD * GN_THREADS) {         // (every load is made, behind the last value that again)
+    T v[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) v[u] = x[o + u * GN_THREADS < end ? o + u * GN_THREADS : end - 1];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (o + u * GN_THREADS < end) add(to_f32<T>(v[u]));
+  }
   sum = block_sum<GN_THREADS>(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
