@@ -758,8 +758,9 @@ int dispatch(BalanceArgs a, FinishArgs* finish, int dtype, hipStream_t s) {
 
 int check_shape(const char* who, const void* x, int dtype, long groups, long rows, int experts) {
   RM_REQUIRE(dtype == REPMODE_F32 || dtype == REPMODE_BF16, "%s: bad dtype %d", who, dtype);
-  RM_REQUIRE(groups > 0 && groups <= 65535 && rows >= 0 && rows < (1L << 31) && experts > 0 && experts <= BL_MAX_E,
-             "%s: 1..65535 groups of less than 2^31 rows, 1..%d experts; got %ld groups of %ld rows over %d experts", who, BL_MAX_E, groups, rows, experts);
+  RM_REQUIRE(groups > 0 && groups <= 65535 && rows >= 0 && experts > 0 && experts <= BL_MAX_E,
+             "%s: 1..65535 groups, 1..%d experts; got %ld groups of %ld rows over %d experts", who, BL_MAX_E, groups, rows, experts);
+  RM_REQUIRE(rows < (1L << 31), "%s: too many rows in a group", who);
   RM_REQUIRE(x || rows == 0, "%s: null pointer", who);
   return REPMODE_OK;
 }
