@@ -2,7 +2,7 @@
 """Summarise rocprofv3 PMC passes (one counter set per pass, as MI355X_MICROARCH.md prescribes) into per-kernel-family HBM
 traffic per launch and MFMA utilisation.
 
-    python profiles/pmc_summary.py <dir with pmc_FETCH_SIZE/, pmc_WRITE_SIZE/, pmc_MFMA/> <batch> <dtype>  > profiles/rNN_pmc_traffic.json
+    python profiles/pmc_summary.py <dir with pmc_FETCH_SIZE/, pmc_WRITE_SIZE/, pmc_MFMA/> <batch> <dtype>  > profiles/step_pmc_traffic.json
 
 FETCH_SIZE / WRITE_SIZE are in KiB.  gfx950 correction (MI355X_MICROARCH.md, HBM section): FETCH_SIZE reports exactly half
 of the bytes of a wide (16 B/lane) coalesced streaming read, which is how these kernels read -> the read side is doubled.

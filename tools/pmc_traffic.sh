@@ -1,5 +1,5 @@
 # HBM traffic per kernel family from rocprofv3 PMC passes (one counter per pass), run through gpurun:
-#   bash tools/pmc_traffic.sh ; python profiles/pmc_summary.py gpurun_out > profiles/rNN_pmc_traffic.json
+#   bash tools/pmc_traffic.sh ; python profiles/pmc_summary.py gpurun_out > profiles/step_pmc_traffic.json
 R=$GRAFT_REPO_ROOT
 cd /tmp && export TMPDIR=/tmp
 for c in FETCH_SIZE WRITE_SIZE; do
