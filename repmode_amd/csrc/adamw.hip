@@ -19,8 +19,8 @@
 //
 // What bounds both: HBM.  float32 moments move 28 B an element (bfloat16 parameters: 22), 8-bit ones 16 (10).  108.6 M float32 parameters
 // 517 us (5.9 TB/s; four reads and three writes without arithmetic reach that too) and, 8-bit moments, 283 us (6.1); 201 M bfloat16
-// ones 755 us (5.9), 402.8 M with 8-bit moments 697 us (5.8).  With bfloat16 parameters and 8-bit moments the vector units are next:
-// hence one hash multiplication for four elements, and the hardware's stochastic conversions.
+// ones 750 us (5.9), 402.8 M with 8-bit moments 670 us (6.0).  With bfloat16 parameters and 8-bit moments the vector units are next:
+// hence one first hash multiplication for four elements, and the hardware's stochastic conversions.
 #include "common.h"
 
 #include <cmath>
@@ -140,7 +140,12 @@ __device__ __forceinline__ void store4(uint8_t* p, uint32_t x, int left) {
 // The random bits mix32(index ^ key) of a lane's four elements, j = 0, 4, .. of a chunk that starts at a multiple of AW_CHUNK (a power
 // of two below 2^16).  There the first round's x ^ (x >> 16) is s ^ j with one s for the whole chunk, and its product
 // with the odd factor differs between the four elements by multiples of that factor which are the chunk's too: one multiplication
-// instead of four.
+// instead of four.  (held(): the compiler is not to see where a value comes from.  It would undo this, and make a product that is shifted
+// afterwards a second product; integer products take several times an addition's time.)
+__device__ __forceinline__ uint32_t held(uint32_t x) {
+  asm("" : "+v"(x));
+  return x;
+}
 struct Noise {
   uint32_t s, c[4];
   __device__ __forceinline__ Noise(uint32_t chunk, uint32_t key) {
@@ -150,11 +155,11 @@ struct Noise {
     for (int k = 0; k < 4; ++k) c[k] = ((t & 3u) ^ k) * 0x455c2ed3u;
   }
   __device__ __forceinline__ void operator()(uint32_t j, uint32_t (&h)[4]) const {
-    const uint32_t product = (s ^ j) * 0x455c2ed3u;
+    const uint32_t product = held((s ^ j) * 0x455c2ed3u);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint32_t z = product + c[k];
-      z = (z ^ (z >> 15)) * 0x55a35cd1u;
+      z = held((z ^ (z >> 15)) * 0x55a35cd1u);
       h[k] = z ^ (z >> 16);
     }
   }
@@ -182,7 +187,8 @@ __device__ __forceinline__ void store4_param(bf16_t* p, const f32x4& x, int left
 
 // m, v: one rounding per operation.  p: square root and reciprocal of the hardware (1 ulp each; they take numbers below 2^-126 for zero,
 // so such a v goes through a square root of 2^100 v).
-__device__ __forceinline__ void update(const AdamWHyper& h, float clip, f32x4& p, const f32x4& grad, f32x4& m, f32x4& v, float v_scale) {
+// Returns the bits, less one, of the smallest v above zero.
+__device__ __forceinline__ uint32_t update(const AdamWHyper& h, float clip, f32x4& p, const f32x4& grad, f32x4& m, f32x4& v, float v_scale) {
   const float b = h.beta2 * v_scale;
   uint32_t least = ~0u;
 #pragma unroll
@@ -202,6 +208,7 @@ __device__ __forceinline__ void update(const AdamWHyper& h, float clip, f32x4& p
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) p[k] = fmaf(-(h.step * m[k]), __builtin_amdgcn_rcpf(fmaf(root[k], h.root, h.eps)), p[k] * h.decay);
+  return least;
 }
 
 // the values of 4 e4m3 / e5m2 codes
@@ -250,7 +257,12 @@ __device__ __forceinline__ uint32_t encode_special(float x, uint32_t code, bool 
 
 // A block's m and v as codes.  The conversions round stochastically by adding the upper 20 (e4m3) or 21 (e5m2) bits of their second
 // operand to the part cut off -- also below the smallest normal value -- which is this file's rounding with 16 random bits and a half.
-__device__ __forceinline__ void encode4(const f32x4& m, const f32x4& v, const uint32_t (&h)[4], uint32_t& mw, uint32_t& vw, uint32_t& me, uint32_t& ve) {
+// least_v: at most the bits, less one, of the lane's smallest v above zero.  RARE: a v that would be rounded to zero is looked for before
+// all are guarded against it (with bfloat16 parameters, where the vector units are as busy as HBM: 402.8 M of them 711 us, without the
+// branch 737; with float32 ones they are not, and the branch costs: 108.6 M 287 us, without 283).
+template <bool RARE>
+__device__ __forceinline__ void encode4(const f32x4& m, const f32x4& v, uint32_t least_v, const uint32_t (&h)[4], uint32_t& mw, uint32_t& vw,
+                                        uint32_t& me, uint32_t& ve) {
   uint32_t most_m = largest(m, ~0u), most_v = largest(v, ~0u);
   const bool finite = most_m < 0x7f800000u && most_v < 0x7f800000u;           // (of the whole block)
   if (!finite) { most_m = largest(m, 0x7f800000u); most_v = largest(v, 0x7f800000u); }
@@ -262,9 +274,13 @@ __device__ __forceinline__ void encode4(const f32x4& m, const f32x4& v, const ui
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     x[k] = m[k] * mi;
-    y[k] = fmaxf(v[k] * vi, v[k] > 0.f ? 0x1p-16f : 0.f);                     // (above zero: not rounded to zero)
+    y[k] = v[k] * vi;
     a[k] = (h[k] << 16) | 0x8000u;
     b[k] = (h[k] & 0xffff0000u) | 0x8000u;
+  }
+  if (!RARE || __any(ve <= 16 || least_v < ((ve - 16) << 23))) {             // (above zero: not rounded to zero)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = fmaxf(y[k], v[k] > 0.f ? 0x1p-16f : 0.f);
   }
   int p = 0, q = 0;
   p = __builtin_amdgcn_cvt_sr_fp8_f32(x[0], a[0], p, 0);
@@ -327,7 +343,7 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
     if constexpr (EIGHT) {
       const uint32_t me0 = __builtin_amdgcn_readfirstlane(ME[u]), ve0 = __builtin_amdgcn_readfirstlane(VE[u]);
       f32x4 m4 = decode_e4m3(M[u]) * power_of_two(me0), v4 = decode_e5m2(V[u]);
-      update(h, clip, P[u], G[u], m4, v4, power_of_two(ve0));
+      const uint32_t least_v = update(h, clip, P[u], G[u], m4, v4, power_of_two(ve0));
       if constexpr (HOW == AW_PART) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -335,7 +351,7 @@ __device__ __forceinline__ void adamw_units(const AdamWArgs& a, int i, const Ada
       }
       uint32_t r[4], mw, vw, me, ve;
       state_noise(j, r);
-      encode4(m4, v4, r, mw, vw, me, ve);
+      encode4<sizeof(T) == 2>(m4, v4, least_v, r, mw, vw, me, ve);
       store4_param<HOW>(p, P[u], left, param_noise, j);
       store4<HOW>(m, mw, left);
       store4<HOW>(v, vw, left);
