@@ -545,6 +545,32 @@ def test_adamw8_zero_state_and_zero_gradients():
     assert bool((p > 0.9).all()) and bool((p <= 1.0).all())
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_adamw8_second_moments_near_zero(dtype):
+    """Blocks whose second moments span what e5m2 does not, that underflow as a whole, or that are alike: every code by the definition, and
+    none above zero becomes zero."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(8)
+    g = torch.randn(7, 256, generator=gen)
+    g[0] *= torch.logspace(-12, 0, 256)                  # beside ordinary ones
+    g[1, 1:] = 0.0                                       # one value and zeros
+    g[2, :200] *= 1e-7
+    g[3] *= 1e-19                                        # squares below the normal range
+    g[4] *= 1e-25                                        # squares that are zero
+    g[5, 100] = 1e15
+    g = g.reshape(-1)[:7 * 256 - 31].to(dtype)
+    p = torch.zeros(g.numel(), device=DEV, dtype=dtype)
+    m, e, v, f = ops.adamw8_state(p)
+    ops.adamw8_step([p], [g.to(DEV)], [m], [e], [v], [f], 1, seed=21, **HYPER)
+    f32 = lambda x: torch.tensor(x, dtype=torch.float32)
+    gi = g.float()
+    v1 = torch.zeros(()) * f32(HYPER['betas'][1]) + f32(1 - HYPER['betas'][1]) * gi * gi
+    h, _ = _noise(21, 1, 0, torch.arange(g.numel()))
+    wv, ev, _ = _encode(v1.double(), ((h >> 16).double() + 0.5) / 65536, 2, -14, 14, 2.0 ** -16)
+    assert torch.equal(_bytes(f).double() - 127, ev) and torch.equal(_decode(v, f), wv)
+    assert bool(((wv > 0) == (v1 > 0)).all()) and int((v1 == 0).sum()) > 400
+
+
 def test_adamw8_follows_the_gradients():
     """What rounding to the nearest would lose: with beta2 = 0.999 every step moves v by far less than half of a code's step, and
     the mean of v still follows 1 - 0.999^t (its deviation over 65536 elements is below 1 %)."""
