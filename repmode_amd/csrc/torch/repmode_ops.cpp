@@ -1839,30 +1839,34 @@ std::tuple<Tensor, Tensor> op_grad_norm(const TensorList& tensors, double max_no
   TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
   TORCH_CHECK(max_norm >= 0, "grad_norm: max_norm must not be negative or NaN, got ", max_norm);
   const size_t n = tensors.size();
+  require_hip(tensors.get(0), "grad_norm: tensor");
   const at::Device dev = tensors.get(0).device();
-  for (size_t i = 0; i < n; ++i) {
-    const Tensor& t = tensors.get(i);
-    require_hip(t, "grad_norm: tensor");
-    TORCH_CHECK(t.layout() == at::kStrided, "grad_norm: tensor ", i, " is not strided");
-    (void)dtype_code(t.scalar_type());
-    TORCH_CHECK(t.device() == dev, "grad_norm: tensor ", i, " is on ", t.device(), ", tensor 0 on ", dev);
-  }
   DeviceGuard guard(dev);
   at::NoGradGuard no_grad;
   std::vector<const void*> x[2];
   std::vector<long> numel[2];
   std::vector<Tensor> hold;
   long room = 0;
-  for (int code : {REPMODE_F32, REPMODE_BF16}) { x[code].reserve(n); numel[code].reserve(n); }
   for (size_t i = 0; i < n; ++i) {
     const Tensor& t = tensors.get(i);
-    if (t.numel() == 0) continue;
-    if (!t.is_non_overlapping_and_dense()) hold.push_back(t.contiguous());        // (any order of the elements has the same norm)
+    if (t.device() != dev) {
+      require_hip(t, "grad_norm: tensor");
+      TORCH_CHECK(false, "grad_norm: tensor ", i, " is on ", t.device(), ", tensor 0 on ", dev);
+    }
+    TORCH_CHECK(t.layout() == at::kStrided, "grad_norm: tensor ", i, " is not strided");
     const int code = dtype_code(t.scalar_type());
-    x[code].push_back((t.is_non_overlapping_and_dense() ? t : hold.back()).data_ptr());
-    numel[code].push_back((long)t.numel());
+    const long count = (long)t.numel();
+    if (count == 0) continue;
+    if (x[code].empty()) { x[code].reserve(n - i); numel[code].reserve(n - i); }
+    if (t.is_non_overlapping_and_dense()) {
+      x[code].push_back(t.const_data_ptr());
+    } else {
+      hold.push_back(t.contiguous());                          // (any order of the elements has the same norm)
+      x[code].push_back(hold.back().const_data_ptr());
+    }
+    numel[code].push_back(count);
     const long per = REPMODE_GRAD_NORM_CHUNK / (code == REPMODE_F32 ? 4 : 2);
-    room += (t.numel() + per - 1) / per;
+    room += (count + per - 1) / per;
   }
   auto f32 = tensors.get(0).options().dtype(at::kFloat).requires_grad(false);
   Tensor norm = at::empty({}, f32), clip = at::empty({}, f32), partial = at::empty({std::max(room, 1L)}, f32.dtype(at::kDouble));
