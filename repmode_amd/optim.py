@@ -158,6 +158,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError('repmode_amd.optim.AdamW: max_norm must be positive, got %r' % (max_norm,))
         self.max_norm, self.seed, self.device_step, self.last_norm = max_norm, int(seed), bool(capturable), None
         self._step_dev = {}          # group index -> int64[1] on the device (capturable)
+        self._captured = False       # a step was captured: some graph may hold moments and counts by address
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_numel=min_8bit_numel))
 
@@ -170,7 +171,7 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):
         self.sync_steps()
         return {**super().__getstate__(), 'max_norm': self.max_norm, 'seed': self.seed, 'device_step': self.device_step, 'last_norm': None,
-                '_step_dev': {}}
+                '_step_dev': {}, '_captured': False}
 
     def _state(self, p, group):
         st = self.state[p]
@@ -199,7 +200,34 @@ class AdamW(torch.optim.Optimizer):
         self.sync_steps()
         return super().state_dict()
 
+    @staticmethod
+    def _kept_as(v):
+        """The type a saved moment is kept in: float32 for anything of 16 bits (a stock optimizer's of bfloat16 parameters)."""
+        return torch.float32 if v.dtype in (torch.bfloat16, torch.float16) else v.dtype
+
+    def _check_captured(self, state_dict):
+        """Whether a state can go into the tensors that a captured step holds; raises before anything has changed where it cannot."""
+        for saved, group in zip(state_dict['param_groups'], self.param_groups):
+            counts = set()
+            for key, p in zip(saved['params'], group['params']):
+                st, there = state_dict['state'].get(key, {}), self.state.get(p, {})
+                if st or there:
+                    counts.add(int(st.get('step', 0)))
+                if not st or not there:                  # (no moments yet; or none saved: those that are there become zero)
+                    continue
+                new = {k: (self._kept_as(v), v.shape) for k, v in st.items() if k != 'step' and torch.is_tensor(v)}
+                if new != {k: (t.dtype, t.shape) for k, t in there.items() if k != 'step'}:
+                    raise ValueError('repmode_amd.optim.AdamW: a captured step holds this optimizer\'s moments, and the state has others (another '
+                                     'number of bits, other shapes): load it into a new optimizer and capture again')
+            if len(counts) > 1:
+                raise ValueError('repmode_amd.optim.AdamW: a captured step holds one step count for a group, and the state\'s counts differ: load it '
+                                 'into a new optimizer and capture again')
+
     def load_state_dict(self, state_dict):
+        """As torch.optim.AdamW's, with the moments as they were saved.  After a captured step the state goes into the tensors that the
+        graph holds -- a parameter without state gets zero moments -- and one that does not fit them is refused."""
+        if self._captured:
+            self._check_captured(state_dict)
         own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel')} for g in self.param_groups]
         # (captured steps hold the moments by address, as they do the step counts: what fits goes into the tensors that are there)
         held = {p: dict(st) for p, st in self.state.items()} if self.device_step else {}
@@ -215,18 +243,31 @@ class AdamW(torch.optim.Optimizer):
                     if k == 'step':
                         self.state[p][k] = torch.tensor(float(v))
                     elif torch.is_tensor(v):
-                        v = v.detach().to(p.device, copy=True)
-                        v = v.float() if v.dtype in (torch.bfloat16, torch.float16) else v
+                        v = v.detach().to(p.device, self._kept_as(v), copy=True)
                         there = held.get(p, {}).get(k)
                         if torch.is_tensor(there) and there.dtype == v.dtype and there.shape == v.shape:
                             v = there.copy_(v)
                         self.state[p][k] = v
+                if self._captured and held.get(p) and not self.state.get(p):
+                    self.state[p] = held[p]
+                    self._rewind(held[p])
         for gi, dev in list(self._step_dev.items()):
             counts = {int(self.state[p]['step']) for p in self.param_groups[gi]['params'] if 'step' in self.state.get(p, {})}
             if len(counts) <= 1:
                 dev.fill_(counts.pop() if counts else 0)
-            else:
+            else:                        # (no step was captured: the next one says that they differ)
                 del self._step_dev[gi]
+
+    @staticmethod
+    def _rewind(st):
+        """A parameter's state as before its first step, in place."""
+        for k, t in st.items():
+            if k == 'step':
+                st[k] = torch.tensor(0.0)
+            elif t.dtype == torch.float32:
+                t.zero_()
+            else:
+                t.view(torch.uint8).fill_(127 if t.dtype == torch.float8_e8m0fnu else 0)
 
     def _count_on_device(self, gi, steps, device):
         """The group's step count on the device; ``steps``: its parameters' host counters, which go on as well."""
@@ -270,6 +311,7 @@ class AdamW(torch.optim.Optimizer):
             states = [self._state(p, group) for p in ps]
             if self.device_step:
                 calls = [(self._count_on_device(gi, [st['step'] for st in states], ps[0].device), range(len(ps)))]
+                self._captured |= _capturing()
             else:
                 # parameters that have seen the same number of updates go together (normally: all of them)
                 if torch.is_tensor(group['lr']):

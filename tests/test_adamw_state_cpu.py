@@ -1,0 +1,115 @@
+"""optim.AdamW's state where a captured step holds it by address, without a GPU: the kernels are replaced, a capture is pretended."""
+import copy
+
+import pytest
+import torch
+
+from test_train_ops_cpu import _FakeOps
+
+
+def _captured(monkeypatch, sizes=(5000, 7), groups=None, **kw):
+    """An optimizer after one step launch by launch and one that was captured, and its parameters."""
+    from repmode_amd import ops, optim
+    monkeypatch.setattr(ops, 'list_ops', lambda: _FakeOps())
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in sizes]
+    opt = optim.AdamW(groups(ps) if groups else ps, capturable=True, **kw)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    with monkeypatch.context() as m:
+        m.setattr(optim, '_capturing', lambda: True)
+        opt.step()
+    return opt, ps
+
+
+def _tensors(opt, ps):
+    return {(i, k): t for i, p in enumerate(ps) for k, t in opt.state[p].items() if k != 'step'}
+
+
+def _loaded(bits, sizes=(5000, 7), steps=(3, 3)):
+    """A state dict of an optimizer of that many bits whose moments are not zero."""
+    from repmode_amd import ops, optim
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in sizes]
+    opt = optim.AdamW(ps, state_bits=bits)
+    for p, n in zip(ps, steps):
+        opt._state(p, opt.param_groups[0])['step'] = torch.tensor(float(n))
+        for k, t in opt.state[p].items():
+            if k != 'step':
+                t.view(torch.uint8).fill_(60)
+    return opt.state_dict()
+
+
+def _bytes(t):
+    return t.reshape(-1).view(torch.uint8)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_state_goes_into_what_a_captured_step_holds(monkeypatch, bits):
+    opt, ps = _captured(monkeypatch, state_bits=bits)
+    held, count = _tensors(opt, ps), opt._step_dev[0]
+    saved = _loaded(bits)
+    opt.load_state_dict(copy.deepcopy(saved))
+    now = _tensors(opt, ps)
+    assert sorted(now) == sorted(held) and all(now[k] is held[k] for k in held) and opt._step_dev[0] is count and int(count) == 3
+    for i, p in enumerate(ps):
+        for k, t in saved['state'][i].items():
+            if k != 'step':
+                assert torch.equal(_bytes(opt.state[p][k]), _bytes(t))
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_dict_without_state_rewinds_what_a_captured_step_holds(monkeypatch, bits):
+    """What a new optimizer's state dict has: no moments, no counts.  Zero moments, zero codes with the scale 1."""
+    from repmode_amd import ops, optim
+    opt, ps = _captured(monkeypatch, state_bits=bits)
+    opt.load_state_dict(copy.deepcopy(_loaded(bits)))
+    held, count = _tensors(opt, ps), opt._step_dev[0]
+    opt.load_state_dict(optim.AdamW([torch.nn.Parameter(p.detach().clone()) for p in ps], state_bits=bits).state_dict())
+    now = _tensors(opt, ps)
+    assert sorted(now) == sorted(held) and all(now[k] is held[k] for k in held) and opt._step_dev[0] is count and int(count) == 0
+    for p in ps:
+        fresh = dict(zip(('exp_avg', 'exp_avg_scale', 'exp_avg_sq', 'exp_avg_sq_scale'), ops.adamw8_state(p)))
+        for k, t in opt.state[p].items():
+            if k == 'step':
+                assert int(t) == 0
+            else:
+                assert torch.equal(_bytes(t), _bytes(fresh[k]) if t.dtype != torch.float32 else torch.zeros(4 * p.numel(), dtype=torch.uint8)), k
+
+
+@pytest.mark.parametrize('have, loads', [(8, 32), (32, 8)])
+def test_moments_of_other_bits_are_refused_under_a_captured_step(monkeypatch, have, loads):
+    opt, ps = _captured(monkeypatch, state_bits=have)
+    held, before = _tensors(opt, ps), copy.deepcopy(opt.state_dict())
+    with pytest.raises(ValueError, match='captured'):
+        opt.load_state_dict(_loaded(loads))
+    now, after = _tensors(opt, ps), opt.state_dict()
+    assert all(now[k] is held[k] for k in held) and after['param_groups'] == before['param_groups']
+    for i, st in before['state'].items():
+        assert all(torch.equal(_bytes(t), _bytes(after['state'][i][k])) for k, t in st.items())
+
+
+def test_other_shapes_and_counts_that_differ_are_refused_under_a_captured_step(monkeypatch):
+    opt, ps = _captured(monkeypatch)
+    held, count = _tensors(opt, ps), opt._step_dev[0]
+    for saved in (_loaded(32, sizes=(5001, 7)), _loaded(32, steps=(3, 4))):
+        with pytest.raises(ValueError, match='captured'):
+            opt.load_state_dict(saved)
+    half = _loaded(32)
+    del half['state'][1]                                 # (one parameter at step 3, the other at none)
+    with pytest.raises(ValueError, match='captured'):
+        opt.load_state_dict(half)
+    assert all(t is held[k] for k, t in _tensors(opt, ps).items()) and opt._step_dev[0] is count and int(count) == 0
+
+
+@pytest.mark.parametrize('have, loads', [(8, 32), (32, 8)])
+def test_before_a_capture_moments_keep_the_bits_they_were_saved_with(monkeypatch, have, loads):
+    """Nothing holds them yet: as without ``capturable``."""
+    from repmode_amd import ops, optim
+    monkeypatch.setattr(ops, 'list_ops', lambda: _FakeOps())
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in (5000, 7)]
+    opt = optim.AdamW(ps, capturable=True, state_bits=have)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    opt.load_state_dict(_loaded(loads))
+    assert ('exp_avg_scale' in opt.state[ps[0]]) == (loads == 8) and int(opt._step_dev[0]) == 3
