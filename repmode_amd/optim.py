@@ -145,7 +145,8 @@ class AdamW(torch.optim.Optimizer):
     set per group.
     ``seed``: of the stochastic roundings (8-bit moments, bfloat16 parameters); a run with the same seed repeats itself.
     ``capturable``: the step count of each group lives on the device, so that ``step()`` can be part of a captured HIP graph (after
-    one step launch by launch); a group's ``lr`` may then be a float32 tensor of one value on the device, which replays read.
+    one step launch by launch); a group's ``lr`` may then be a float32 tensor of one value on the device, which replays read (every other
+    setting, and an ``lr`` that is a number, stays what it was at the capture).
 
     The state of a float32 parameter with 32-bit moments is ``torch.optim.AdamW``'s (``step``, ``exp_avg``, ``exp_avg_sq``): their state
     dicts interchange.  Loaded moments keep the bits they were saved with.  No CPU path."""
@@ -225,16 +226,23 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch.optim.AdamW's, with the moments as they were saved.  After a captured step the state goes into the tensors that the
-        graph holds -- a parameter without state gets zero moments -- and one that does not fit them is refused."""
+        graph holds -- a parameter without state gets zero moments -- and one that does not fit them is refused.  A group's learning rate
+        on the device stays the tensor that it is and takes the loaded value."""
         if self._captured:
             self._check_captured(state_dict)
-        own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel')} for g in self.param_groups]
+        own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel', 'lr')} for g in self.param_groups]
         # (captured steps hold the moments by address, as they do the step counts: what fits goes into the tensors that are there)
         held = {p: dict(st) for p, st in self.state.items()} if self.device_step else {}
         super().load_state_dict(state_dict)
         for group, mine in zip(self.param_groups, own):          # (a stock optimizer's groups have neither)
+            lr = mine.pop('lr')
             for k, v in mine.items():
                 group.setdefault(k, v)
+            if torch.is_tensor(lr):
+                group['lr'] = lr.fill_(float(group['lr']))
+            elif torch.is_tensor(group['lr']):
+                group['lr'] = (group['lr'].to(next(iter(group['params']), group['lr']).device, torch.float32) if self.device_step
+                               else float(group['lr']))
         # (the base class casts floating moments to the parameter's type: 8-bit codes and the float32 moments of bfloat16
         # parameters are taken from the dict as they are)
         for saved, group in zip(state_dict['param_groups'], self.param_groups):

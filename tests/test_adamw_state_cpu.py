@@ -113,3 +113,40 @@ def test_before_a_capture_moments_keep_the_bits_they_were_saved_with(monkeypatch
     opt.step()
     opt.load_state_dict(_loaded(loads))
     assert ('exp_avg_scale' in opt.state[ps[0]]) == (loads == 8) and int(opt._step_dev[0]) == 3
+
+
+@pytest.mark.parametrize('saved_lr', [0.25, torch.tensor(0.25), torch.tensor(0.25, dtype=torch.float64)])
+def test_a_learning_rate_on_the_device_stays_where_it_is(monkeypatch, saved_lr):
+    """The tensor that replays read takes the loaded value, whatever the state has it as; also before a capture."""
+    lr = torch.tensor(0.5)
+    opt, ps = _captured(monkeypatch, groups=lambda p: [dict(params=p[:1], lr=lr), dict(params=p[1:], lr=0.125)])
+    saved = opt.state_dict()
+    saved = dict(saved, param_groups=[dict(g, lr=saved_lr) for g in saved['param_groups']])
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]['lr'] is lr and float(lr) == 0.25 and lr.dtype == torch.float32
+    assert float(opt.param_groups[1]['lr']) == 0.25
+    if torch.is_tensor(saved_lr):                        # (neither the dict's own tensor nor its type)
+        assert opt.param_groups[1]['lr'] is not saved_lr and opt.param_groups[1]['lr'].dtype == torch.float32
+        assert opt.param_groups[1]['lr'].device == ps[0].device
+
+
+def test_a_saved_learning_rate_on_the_device_becomes_a_number_without_capturable(monkeypatch):
+    from repmode_amd import ops, optim
+    monkeypatch.setattr(ops, 'list_ops', lambda: _FakeOps())
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = optim.AdamW([p])
+    saved = opt.state_dict()
+    saved['param_groups'][0]['lr'] = torch.tensor(0.25)
+    opt.load_state_dict(saved)
+    p.grad = torch.ones(3)
+    opt.step()
+    assert opt.param_groups[0]['lr'] == 0.25 and not torch.is_tensor(opt.param_groups[0]['lr'])
+
+
+def test_a_scheduler_fills_the_captured_learning_rate_after_a_load(monkeypatch):
+    lr = torch.tensor(0.5)
+    opt, ps = _captured(monkeypatch, lr=lr)
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda t: 0.5 ** t)
+    sched.step()
+    assert opt.param_groups[0]['lr'] is lr and float(lr) == 0.25
