@@ -509,8 +509,9 @@ int repmode_adam_expert_frags_dev(int nblocks, float* const* p5, const float* co
  *   position    of each tensor in the caller's whole list: with seed and step it decides the stochastic roundings' random bits
  *   step        the 1-based count of this update.  hyper_dev != NULL: a captured step -- lr .. seed are not read, the
  *               constants come from device memory (REPMODE_ADAMW_HYPER_FLOATS floats, 16-byte aligned) as
- *               repmode_adamw_hyper_dev leaves them: it advances *step_dev (int64) and takes lr from lr_dev where that is given.
- *   clip        device scalar or NULL (1).  NaN: parameters and moments stay as they are. */
+ *               repmode_adamw_hyper_clip_dev leaves them: it advances *step_dev (int64) and takes lr from lr_dev where that is given.
+ *   clip        device scalar or NULL (1).  NaN: parameters and moments stay as they are, and *step_dev where
+ *               repmode_adamw_hyper_clip_dev is given the same clip (repmode_adamw_hyper_dev advances it whatever clip is). */
 #define REPMODE_ADAMW_MAX 60
 #define REPMODE_ADAMW_BLOCK 256
 #define REPMODE_ADAMW_HYPER_FLOATS 8
@@ -520,6 +521,8 @@ int repmode_adamw_multi(int ntensors, int dtype, int state_bits, void* const* p,
                         const float* hyper_dev, const float* clip, void* stream);
 int repmode_adamw_hyper_dev(long* step_dev, float* hyper_dev, double lr, const float* lr_dev, double beta1, double beta2, double eps,
                             double weight_decay, unsigned long seed, void* stream);
+int repmode_adamw_hyper_clip_dev(long* step_dev, float* hyper_dev, double lr, const float* lr_dev, double beta1, double beta2,
+                                 double eps, double weight_decay, unsigned long seed, const float* clip, void* stream);
 
 /* ---- the norm of many tensors together (csrc/grad_norm.hip) ----
  * partial: writes one float64 sum of squares per REPMODE_GRAD_NORM_CHUNK bytes (or part of them) of every tensor into

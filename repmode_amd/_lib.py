@@ -39,6 +39,7 @@ _SIGNATURES = {
     'repmode_adam_expert_frags_dev': [_I] + [_P] * 12 + [_P, _P],
     'repmode_adamw_multi': [_I] * 3 + [_P] * 8 + [_c.c_double] * 5 + [_c.c_long, _c.c_ulong, _P, _P, _P],
     'repmode_adamw_hyper_dev': [_P, _P, _c.c_double, _P] + [_c.c_double] * 4 + [_c.c_ulong, _P],
+    'repmode_adamw_hyper_clip_dev': [_P, _P, _c.c_double, _P] + [_c.c_double] * 4 + [_c.c_ulong, _P, _P],
     'repmode_grad_norm_partial': [_I, _I, _P, _P, _P, _c.c_long, _P, _P],
     'repmode_grad_norm_finish': [_P, _c.c_long, _c.c_double, _P, _P, _P],
     'repmode_balance_plan': [_c.c_long, _c.c_long, _I, _P],

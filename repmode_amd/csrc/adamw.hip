@@ -4,7 +4,7 @@
 //     m <- m + (1 - beta1) (g' - m)
 //     v <- v beta2 + (1 - beta2) g' g'
 //     p <- p (1 - lr wd) - (lr / (1 - beta1^t)) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
-// A clip factor that is NaN (gradients that are not finite) leaves parameters and moments as they were.
+// A clip factor that is NaN (gradients that are not finite) leaves parameters, moments and a count on the device as they were.
 //
 // 8-bit moments.  256 consecutive elements of a tensor (flat order) are a block; a block's m is held as e4m3 values and its v as
 // e5m2 values, each times a power of two of its own (e8m0: one byte a block).  The powers are taken from the block's largest
@@ -412,12 +412,13 @@ int check_hyper(double lr, double beta1, double beta2, double eps, double weight
 // (an eps above zero stays so: the reciprocal takes what is below 2^-126 for zero)
 __host__ __device__ __forceinline__ float float_eps(double eps) { return eps > 0 && eps < 0x1p-126 ? 0x1p-126f : (float)eps; }
 
-// one thread: *step_dev += 1, and the constants of that step in the host path's double arithmetic
+// one thread: *step_dev += 1 unless the step is left out, and the constants of that step in the host path's double arithmetic
 __global__ void adamw_hyper_kernel(long* __restrict__ step_dev, AdamWHyper* __restrict__ out, double lr, const float* __restrict__ lr_dev,
-                                   double beta1, double beta2, double eps, double weight_decay, uint64_t seed) {
+                                   double beta1, double beta2, double eps, double weight_decay, uint64_t seed,
+                                   const float* __restrict__ clip) {
   if (threadIdx.x != 0 || blockIdx.x != 0) return;
   const long t = *step_dev + 1;
-  *step_dev = t;
+  if (!clip || *clip == *clip) *step_dev = t;
   const double l = lr_dev ? (double)*lr_dev : lr;
   const double bc1 = 1.0 - pow(beta1, (double)t), bc2 = 1.0 - pow(beta2, (double)t);
   out->w1 = (float)(1.0 - beta1);
@@ -432,15 +433,20 @@ __global__ void adamw_hyper_kernel(long* __restrict__ step_dev, AdamWHyper* __re
 
 }  // namespace
 
-extern "C" int repmode_adamw_hyper_dev(long* step_dev, float* hyper_dev, double lr, const float* lr_dev, double beta1, double beta2,
-                                       double eps, double weight_decay, unsigned long seed, void* stream) {
+extern "C" int repmode_adamw_hyper_clip_dev(long* step_dev, float* hyper_dev, double lr, const float* lr_dev, double beta1, double beta2,
+                                            double eps, double weight_decay, unsigned long seed, const float* clip, void* stream) {
   RM_REQUIRE(step_dev && hyper_dev, "adamw_hyper_dev: null pointer");
-  RM_REQUIRE(((uintptr_t)step_dev & 7) == 0 && ((uintptr_t)hyper_dev & 15) == 0 && ((uintptr_t)lr_dev & 3) == 0, "adamw_hyper_dev: misaligned buffers");
+  RM_REQUIRE(((uintptr_t)step_dev & 7) == 0 && ((uintptr_t)hyper_dev & 15) == 0 && (((uintptr_t)lr_dev | (uintptr_t)clip) & 3) == 0,
+             "adamw_hyper_dev: misaligned buffers");
   if (int rc = check_hyper(lr, beta1, beta2, eps, weight_decay)) return rc;
   hipLaunchKernelGGL(adamw_hyper_kernel, dim3(1), dim3(64), 0, static_cast<hipStream_t>(stream), step_dev, reinterpret_cast<AdamWHyper*>(hyper_dev),
-                     lr, lr_dev, beta1, beta2, eps, weight_decay, (uint64_t)seed);
+                     lr, lr_dev, beta1, beta2, eps, weight_decay, (uint64_t)seed, clip);
   RM_LAUNCH_CHECK("adamw_hyper_dev");
   return REPMODE_OK;
+}
+extern "C" int repmode_adamw_hyper_dev(long* step_dev, float* hyper_dev, double lr, const float* lr_dev, double beta1, double beta2,
+                                       double eps, double weight_decay, unsigned long seed, void* stream) {
+  return repmode_adamw_hyper_clip_dev(step_dev, hyper_dev, lr, lr_dev, beta1, beta2, eps, weight_decay, seed, nullptr, stream);
 }
 
 extern "C" int repmode_adamw_multi(int ntensors, int dtype, int state_bits, void* const* p, const void* const* g, void* const* m, void* const* m_scale,

@@ -1965,8 +1965,8 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
   const float* hd = nullptr;
   if (captured) {
     hyper = at::empty({REPMODE_ADAMW_HYPER_FLOATS}, params.get(0).options().dtype(at::kFloat));
-    RM_CALL(repmode_adamw_hyper_dev, reinterpret_cast<long*>(step_dev->data_ptr<int64_t>()), hyper.data_ptr<float>(), lr,
-            lr_on_dev ? lr_dev->data_ptr<float>() : nullptr, beta1, beta2, eps, weight_decay, (unsigned long)seed, stream_handle());
+    RM_CALL(repmode_adamw_hyper_clip_dev, reinterpret_cast<long*>(step_dev->data_ptr<int64_t>()), hyper.data_ptr<float>(), lr,
+            lr_on_dev ? lr_dev->data_ptr<float>() : nullptr, beta1, beta2, eps, weight_decay, (unsigned long)seed, clip_p, stream_handle());
     hd = hyper.data_ptr<float>();
   }
   // (also where a launch fails half way: some parameters have changed)
