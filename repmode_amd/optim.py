@@ -11,6 +11,8 @@ next forward pass has no layout launch.  No CPU path: parameters must live on th
 ``AdamW`` is for what the reference does not train with: decoupled weight decay, clipping by the gradients' common norm, bfloat16
 parameters and moments in 8 bits.
 """
+import math
+
 import torch
 
 
@@ -139,7 +141,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``max_norm``: the gradients of all groups together are scaled by ``min(1, max_norm / (norm + 1e-6))`` on their way into the
     update (``.grad`` itself stays as it is; ``last_norm`` is the norm, a device scalar).  Where a gradient is not finite the step
-    changes no parameter and no moment.
+    is left out: it changes no parameter, no moment and no step count.  (A count on the host learns of it afterwards: the next ``step()``
+    waits until the GPU is past this one's norm and takes it back, as ``sync_steps()`` and ``state_dict()`` do.)
     ``state_bits``: 32, or 8 -- e4m3 / e5m2 values with a power of two for each 256 elements, rounded stochastically: 2 bytes a
     parameter instead of 8.  Tensors of fewer than ``min_8bit_numel`` elements (biases, norms) keep float32 moments.  Both may be
     set per group.
@@ -160,6 +163,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm, self.seed, self.device_step, self.last_norm = max_norm, int(seed), bool(capturable), None
         self._step_dev = {}          # group index -> int64[1] on the device (capturable)
         self._captured = False       # a step was captured: some graph may hold moments and counts by address
+        self._last = self._flag = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       min_8bit_numel=min_8bit_numel))
 
@@ -172,7 +176,7 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self):
         self.sync_steps()
         return {**super().__getstate__(), 'max_norm': self.max_norm, 'seed': self.seed, 'device_step': self.device_step, 'last_norm': None,
-                '_step_dev': {}, '_captured': False}
+                '_step_dev': {}, '_captured': False, '_last': None, '_flag': None}
 
     def _state(self, p, group):
         st = self.state[p]
@@ -189,8 +193,34 @@ class AdamW(torch.optim.Optimizer):
                 st['exp_avg_sq'] = torch.zeros_like(p, dtype=torch.float32)
         return st
 
+    def _watch(self, clip):
+        """Keeps a step's clip factor -- of one on the GPU: what will be on the host behind an event -- and the list of the counters
+        that it moves, for ``_settle``.  Called between norm and update, so that the event does not wait for the update."""
+        event = None
+        if clip.is_cuda:
+            if self._flag is None:
+                self._flag = torch.empty((), dtype=torch.float32, pin_memory=True), torch.cuda.Event()
+            (flag, event), stream = self._flag, torch.cuda.current_stream(clip.device)
+            clip = flag.copy_(clip, non_blocking=True)
+            event.record(stream)
+        self._last = clip, event, []
+        return self._last[2]
+
+    def _settle(self):
+        """Takes the last step back from the host counters of its parameters if it was left out."""
+        if self._last is not None:
+            clip, event, steps = self._last
+            self._last = None
+            if event is not None:
+                event.synchronize()
+            if math.isnan(clip):
+                for s in steps:
+                    s -= 1
+
     def sync_steps(self):
-        """Device step counts -> the host counters of ``state`` (after graph replays, which run no host code).  One read a group."""
+        """What the GPU knows of the step counts -> the host counters of ``state``: device counts (after graph replays, which run no host
+        code; one read a group), and whether the last step was left out."""
+        self._settle()
         for gi, dev in self._step_dev.items():
             t = float(dev.item())
             for p in self.param_groups[gi]['params']:
@@ -230,6 +260,7 @@ class AdamW(torch.optim.Optimizer):
         on the device stays the tensor that it is and takes the loaded value."""
         if self._captured:
             self._check_captured(state_dict)
+        self._settle()
         own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel', 'lr')} for g in self.param_groups]
         # (captured steps hold the moments by address, as they do the step counts: what fits goes into the tensors that are there)
         held = {p: dict(st) for p, st in self.state.items()} if self.device_step else {}
@@ -313,7 +344,9 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError('repmode_amd.optim.AdamW: a captured step needs capturable=True')
         clip = None
         if self.max_norm is not None:
+            self._settle()
             self.last_norm, clip = ops_.grad_norm(grads, self.max_norm)
+        counted = [] if clip is None or self.device_step else self._watch(clip)
         none = torch.empty(0)
         for gi, group, ps in work:
             states = [self._state(p, group) for p in ps]
@@ -327,6 +360,7 @@ class AdamW(torch.optim.Optimizer):
                 by_step = {}
                 for i, st in enumerate(states):
                     st['step'] += 1
+                    counted.append(st['step'])
                     by_step.setdefault(int(st['step']), []).append(i)
                 calls = by_step.items()
             for count, idx in calls:

@@ -150,3 +150,46 @@ def test_a_scheduler_fills_the_captured_learning_rate_after_a_load(monkeypatch):
     sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda t: 0.5 ** t)
     sched.step()
     assert opt.param_groups[0]['lr'] is lr and float(lr) == 0.25
+
+
+class _Skips(_FakeOps):
+    """Gradient norms that are not finite in the steps that are named."""
+
+    def __init__(self, bad):
+        super().__init__()
+        self.bad = bad
+
+    def grad_norm(self, tensors, max_norm):
+        super().grad_norm(tensors, max_norm)
+        return torch.tensor(2.0), torch.tensor(float('nan') if len(self.norms) in self.bad else 0.5)
+
+
+def test_steps_that_are_left_out_are_not_counted(monkeypatch):
+    """Counts on the host: taken back before they are next used, of the parameters that had a gradient in that step."""
+    from repmode_amd import ops, optim
+    fake = _Skips({1, 3, 4, 6})
+    monkeypatch.setattr(ops, 'list_ops', lambda: fake)
+    a, b = (torch.nn.Parameter(torch.zeros(n)) for n in (5, 6))
+    opt = optim.AdamW([a, b], max_norm=1.0)
+    counts = []
+    for t in range(1, 7):
+        a.grad, b.grad = torch.ones(5), None if t == 3 else torch.ones(6)
+        opt.step()
+        counts.append([(c['n'], c['step']) for c in fake.steps])
+        fake.steps.clear()
+    assert counts == [[(2, 1)], [(2, 1)], [(1, 2)], [(2, 2)], [(2, 2)], [(2, 3)]]
+    assert [int(s['step']) for s in opt.state_dict()['state'].values()] == [2, 2]
+    assert [int(s['step']) for s in copy.deepcopy(opt).state.values()] == [2, 2]
+
+
+def test_a_load_forgets_the_step_before_it(monkeypatch):
+    from repmode_amd import ops, optim
+    fake = _Skips({1})
+    monkeypatch.setattr(ops, 'list_ops', lambda: fake)
+    p = torch.nn.Parameter(torch.zeros(5))
+    opt = optim.AdamW([p], max_norm=1.0)
+    p.grad = torch.ones(5)
+    opt.step()
+    opt.load_state_dict(_loaded(32, sizes=(5,), steps=(3,)))
+    opt.step()
+    assert fake.steps[-1]['step'] == 4 and int(opt.state[p]['step']) == 4

@@ -36,3 +36,63 @@ def test_a_step_that_is_left_out_keeps_the_count_on_the_device(bits):
             ops.adamw8_step(q, g, *r, want, clip=clip, seed=3)
         for a, b in zip(p + sum(s, []), q + sum(r, [])):
             assert torch.equal(_bytes(a), _bytes(b)), want
+
+
+def _with_grads(ps, gs, at=None):
+    for p, g in zip(ps, gs):
+        p.grad = g.clone()
+    if at is not None:
+        ps[0].grad[at] = math.inf
+
+
+@pytest.mark.parametrize('capturable', [False, True])
+@pytest.mark.parametrize('bits', [32, 8])
+def test_the_optimizer_does_not_count_steps_that_are_left_out(bits, capturable):
+    """Gradients that are not finite before, between and after ordinary steps: parameters, moments and counts of a twin that never had
+    those steps."""
+    from repmode_amd.optim import AdamW
+    ps, gs, _ = _fresh(bits)
+    make = lambda: [torch.nn.Parameter(p.clone()) for p in ps]
+    a, b = make(), make()
+    opt, twin = (AdamW(q, lr=1e-2, max_norm=1.0, state_bits=bits, seed=5, capturable=capturable) for q in (a, b))
+    for t, bad in enumerate((True, False, True, True, False, False, True)):
+        g = [x * (t + 1) for x in gs]
+        _with_grads(a, g, 7 if bad else None)
+        opt.step()
+        assert math.isfinite(float(opt.last_norm)) != bad
+        if not bad:
+            _with_grads(b, g)
+            twin.step()
+        for p, q in zip(a, b):
+            assert torch.equal(_bytes(p.detach()), _bytes(q.detach())), t
+    for st, want in zip(opt.state_dict()['state'].values(), twin.state_dict()['state'].values()):
+        assert int(st['step']) == 3
+        assert sorted(st) == sorted(want) and all(torch.equal(_bytes(st[k]), _bytes(want[k])) for k in st if k != 'step')
+
+
+def test_a_captured_step_is_left_out_of_its_count():
+    from repmode_amd.optim import AdamW
+    ps, gs, _ = _fresh(32)
+    a, b = ([torch.nn.Parameter(p.clone()) for p in ps] for _ in range(2))
+    opt, twin = AdamW(a, lr=1e-2, max_norm=1.0, capturable=True), AdamW(b, lr=1e-2, max_norm=1.0)
+    _with_grads(a, gs)
+    _with_grads(b, gs)
+    opt.step()
+    twin.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for t, bad in enumerate((False, True, False, True, False)):
+        for p, g in zip(a, gs):
+            p.grad.copy_(g * (t + 2))
+        if bad:
+            a[1].grad[11] = math.nan
+        graph.replay()
+        if not bad:
+            _with_grads(b, [g * (t + 2) for g in gs])
+            twin.step()
+        torch.cuda.synchronize()
+        for p, q in zip(a, b):
+            assert torch.equal(_bytes(p.detach()), _bytes(q.detach())), t
+    assert all(int(s['step']) == 4 for s in opt.state_dict()['state'].values())
