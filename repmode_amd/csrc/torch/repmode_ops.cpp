@@ -1883,19 +1883,33 @@ std::tuple<Tensor, Tensor> op_grad_norm(const TensorList& tensors, double max_no
   return {norm, clip};
 }
 
-// Whether two of the memory ranges share a byte.  Each list is in the order of its tensors, which mostly is that of their addresses.
+// Memory ranges.  A list is in the order of its tensors, which mostly is that of their addresses.
 using Spans = std::vector<std::pair<const char*, const char*>>;
-bool overlap(Spans (&lists)[5]) {
-  Spans all, next;
+void in_order(Spans& l) {
+  if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
+}
+// Whether two of the ranges share a byte; all: every one, in order.
+bool overlap(Spans (&lists)[5], Spans& all) {
+  Spans next;
   for (Spans& l : lists) {
     if (l.empty()) continue;
-    if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
+    in_order(l);
     next.resize(all.size() + l.size());
     std::merge(all.begin(), all.end(), l.begin(), l.end(), next.begin());
     all.swap(next);
   }
   for (size_t i = 1; i < all.size(); ++i)
     if (all[i].first < all[i - 1].second) return true;
+  return false;
+}
+// whether one of the ranges shares a byte with one of `all`, which are in order and apart
+bool touches(Spans& reads, const Spans& all) {
+  in_order(reads);
+  size_t j = 0;
+  for (const auto& r : reads) {
+    while (j < all.size() && all[j].second <= r.first) ++j;
+    if (j < all.size() && all[j].first < r.second) return true;
+  }
   return false;
 }
 
@@ -1910,14 +1924,16 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
                   (exp_avg_scales.empty() || exp_avg_scales.size() == n), "adamw_step: list lengths differ");
   if (n == 0) return;
   const at::Device dev = params.get(0).device();
-  Spans written[5];                                            // p, m, v and the two scales: a list each
+  Spans written[5], reads, all;                                // written: p, m, v and the two scales, a list each
   for (Spans& w : written) w.reserve(n);
+  reads.reserve(n + 1);
   auto span = [&](int list, const Tensor& t) {
     if (t.numel()) written[list].emplace_back(static_cast<const char*>(t.data_ptr()), static_cast<const char*>(t.data_ptr()) + t.nbytes());
   };
   auto same_order = [](const Tensor& t, const Tensor& p) { return t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous()); };
-  std::vector<char> kind(n);                                   // bit 0: bfloat16, bit 1: 8-bit moments; a kernel each
+  std::vector<char> kind(n), copied(n);                        // bit 0: bfloat16, bit 1: 8-bit moments; a kernel each
   int kinds = 0;
+  bool copies = false;
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params.get(i), &g = grads.get(i), &m = exp_avgs.get(i), &v = exp_avg_sqs.get(i);
     const at::ScalarType dt = p.scalar_type(), mt = m.scalar_type();
@@ -1934,6 +1950,12 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
                 "adamw_step: moments of parameter ", i, ": its shape, strides and device");
     if (p.numel() == 0) continue;
     kinds |= 1 << kind[i];
+    if (same_order(g, p)) {
+      const char* from = static_cast<const char*>(g.const_data_ptr());
+      reads.emplace_back(from, from + p.nbytes());
+    } else {
+      copied[i] = copies = true;
+    }
     span(0, p);
     span(1, m);
     span(2, v);
@@ -1948,7 +1970,7 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
     span(4, vs);
   }
   // what is written is written once: a tensor given twice, or two views of the same memory, would race
-  TORCH_CHECK(!overlap(written), "adamw_step: two of the parameters and moments share memory");
+  TORCH_CHECK(!overlap(written, all), "adamw_step: two of the parameters and moments share memory");
   auto one = [&](const OptTensor& t, at::ScalarType want, const char* what) {
     if (!t.has_value() || !t->defined()) return;
     TORCH_CHECK(t->device() == dev && t->scalar_type() == want && t->numel() == 1, "adamw_step: ", what, ": one ", want, " value on the parameters' device");
@@ -1959,6 +1981,9 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
   const bool captured = step_dev.has_value() && step_dev->defined(), lr_on_dev = lr_dev.has_value() && lr_dev->defined();
   TORCH_CHECK(captured || !lr_on_dev, "adamw_step: a learning rate on the device needs the step count on the device too");
   const float* clip_p = clip.has_value() && clip->defined() ? clip->data_ptr<float>() : nullptr;
+  // nor is what is written read by other threads (gradients of another order are copied before the first launch)
+  if (clip_p) reads.emplace_back(reinterpret_cast<const char*>(clip_p), reinterpret_cast<const char*>(clip_p + 1));
+  TORCH_CHECK(!touches(reads, all), "adamw_step: a gradient or the clip factor shares memory with a parameter or a moment");
   DeviceGuard guard(dev);
   at::NoGradGuard no_grad;
   Tensor hyper;
@@ -1977,7 +2002,14 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
         if (const Tensor& t = ps.get(i); !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     }
   } bump{params};
-  std::vector<Tensor> hold;                                    // gradients brought into their parameters' order
+  std::vector<Tensor> hold;                                    // gradients brought into their parameters' order, as they come below
+  for (int k = 0; k < 4; ++k)
+    for (size_t i = 0; i < n && copies; ++i)
+      if (kind[i] == k && copied[i]) {
+        const Tensor& pi = params.get(i);
+        hold.push_back(at::empty_strided(pi.sizes(), pi.strides(), pi.options()).copy_(grads.get(i)));
+      }
+  size_t held = 0;
   for (int k = 0; k < 4; ++k) {
     if (!(kinds >> k & 1)) continue;
     const bool eight = k & 2;
@@ -1992,12 +2024,10 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
       cnt = 0;
     };
     for (size_t i = 0; i < n; ++i) {
-      const Tensor &pi = params.get(i), &gi = grads.get(i);
+      const Tensor& pi = params.get(i);
       if (kind[i] != k || pi.numel() == 0) continue;
-      const bool as_is = same_order(gi, pi);
-      if (!as_is) hold.push_back(at::empty_strided(pi.sizes(), pi.strides(), gi.options()).copy_(gi));
       p[cnt] = pi.data_ptr();
-      g[cnt] = (as_is ? gi : hold.back()).data_ptr();
+      g[cnt] = (copied[i] ? hold[held++] : grads.get(i)).const_data_ptr();
       m[cnt] = exp_avgs.get(i).data_ptr();
       v[cnt] = exp_avg_sqs.get(i).data_ptr();
       ms[cnt] = eight ? exp_avg_scales.get(i).data_ptr() : nullptr;

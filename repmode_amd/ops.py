@@ -407,7 +407,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     in the list, element)``.  ``step``: the 1-based count of this update, or an int64 tensor of one value on the device that the
     call itself advances (a step that is captured into a graph; ``lr`` may then be a float32 tensor of one value too).
     ``clip``: a float32 device scalar that multiplies the gradients (``grad_norm``); NaN leaves everything as it is, a count on the device too.
-    What is written must not share memory (refused), nor gradients with it.  Lists or tuples; no autograd."""
+    What is written must not share memory, nor gradients or ``clip`` with it (refused).  Lists or tuples; no autograd."""
     adamw8_step(params, grads, exp_avgs, [], exp_avg_sqs, [], step, lr, betas, eps, weight_decay, clip, seed)
 
 

@@ -96,3 +96,39 @@ def test_a_captured_step_is_left_out_of_its_count():
         for p, q in zip(a, b):
             assert torch.equal(_bytes(p.detach()), _bytes(q.detach())), t
     assert all(int(s['step']) == 4 for s in opt.state_dict()['state'].values())
+
+
+def test_gradients_that_share_memory_with_what_is_written():
+    """Refused where threads would race; neighbours, gradients that two parameters share and gradients that are copied first are not."""
+    ops = _ops()
+    z = lambda n=64, d=torch.float32: torch.zeros(n, device=DEV, dtype=d)
+    p, g, m, v = z(), z(), z(), z()
+    m8, e8, v8, f8 = ops.adamw8_state(p)
+    wide = z(200)
+    bad = [
+        lambda: ops.adamw_step([p], [p], [m], [v], 1), lambda: ops.adamw_step([p], [m], [m], [v], 1), lambda: ops.adamw_step([p], [v], [m], [v], 1),
+        lambda: ops.adamw_step([wide[:64]], [wide[63:127]], [m], [v], 1), lambda: ops.adamw_step([wide[63:127]], [wide[:64]], [m], [v], 1),
+        lambda: ops.adamw_step([z(), p], [p, z()], [z(), m], [z(), v], 1), lambda: ops.adamw_step([p], [g], [m], [v], 1, clip=p[:1]),
+        lambda: ops.adamw_step([p], [g], [m], [v], 1, clip=v[63]),
+        lambda: ops.adamw8_step([p[:16]], [m8.view(torch.float32)], [m8[:16]], [e8], [v8[:16]], [f8], 1)]
+    for call in bad:
+        with pytest.raises(RuntimeError, match='shares memory'):
+            call()
+    assert float(p.abs().sum() + m.abs().sum() + v.abs().sum() + wide.abs().sum()) == 0
+    q, w = (torch.randn(k, generator=torch.Generator().manual_seed(k)).to(DEV) for k in (64, 200))
+    def step(ps, gs):
+        ms, vs = ([torch.zeros_like(x, dtype=torch.float32) for x in ps] for _ in range(2))
+        ops.adamw_step(ps, gs, ms, vs, 1)
+        return [_bytes(x.clone()) for x in ps + ms + vs]
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))
+    part = lambda x: (x[:64], x[64:128])
+    apart = step([part(w.clone())[0].clone()], [w[64:128].clone()])
+    assert same(step(*[[x] for x in part(w.clone())]), apart)                                    # neighbours
+    assert same(step([q.clone(), w[:64].clone()], [w[64:128]] * 2)[1::2], step([w[:64].clone()], [w[64:128]]))
+    # of another order: as they were at the call, also where parameters of another type are updated first
+    def mixed():
+        a, b = q.clone().view(8, 8), q[:16].bfloat16()
+        return [a, b], [a.t(), a.view(-1).view(torch.bfloat16)[1::2][:16]]
+    ps, gs = mixed()
+    gs = [g.clone(memory_format=torch.contiguous_format) for g in gs]
+    assert same(step(*mixed()), step(ps, gs))
