@@ -1993,15 +1993,17 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
     RM_CALL(repmode_adamw_hyper_clip_dev, reinterpret_cast<long*>(step_dev->data_ptr<int64_t>()), hyper.data_ptr<float>(), lr,
             lr_on_dev ? lr_dev->data_ptr<float>() : nullptr, beta1, beta2, eps, weight_decay, (unsigned long)seed, clip_p, stream_handle());
     hd = hyper.data_ptr<float>();
+    if (!step_dev->is_inference()) step_dev->unsafeGetTensorImpl()->bump_version();
   }
   // (also where a launch fails half way: some parameters have changed)
   struct Bump {
-    const TensorList& ps;
+    const TensorList* lists[5];
     ~Bump() {
-      for (size_t i = 0; i < ps.size(); ++i)
-        if (const Tensor& t = ps.get(i); !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+      for (const TensorList* l : lists)
+        for (const Tensor* t : l->t)
+          if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     }
-  } bump{params};
+  } bump{{&params, &exp_avgs, &exp_avg_sqs, &exp_avg_scales, &exp_avg_sq_scales}};
   std::vector<Tensor> hold;                                    // gradients brought into their parameters' order, as they come below
   for (int k = 0; k < 4; ++k)
     for (size_t i = 0; i < n && copies; ++i)

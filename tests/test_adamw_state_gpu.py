@@ -132,3 +132,21 @@ def test_gradients_that_share_memory_with_what_is_written():
     ps, gs = mixed()
     gs = [g.clone(memory_format=torch.contiguous_format) for g in gs]
     assert same(step(*mixed()), step(ps, gs))
+
+
+def test_what_is_written_moves_its_version():
+    """Parameters, moments and scales; autograd then refuses a graph that has saved one of them.  Gradients are only read."""
+    ops = _ops()
+    for bits in (32, 8):
+        p, g, s = _fresh(bits)
+        w = torch.ones(5000, device=DEV, requires_grad=True)
+        graph = (w * s[0][0].float()).sum() if bits == 8 else (w * s[0][0]).sum()
+        written = [t for t in p + sum(s, []) if t.numel()]
+        was, read = [t._version for t in written], [t._version for t in g]
+        count = torch.zeros(1, dtype=torch.int64, device=DEV)
+        written, was = written + [count], was + [count._version]
+        ops.adamw8_step(p, g, *s, count)
+        assert all(t._version > v for t, v in zip(written, was)) and [t._version for t in g] == read
+        if bits == 32:
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                graph.backward()
