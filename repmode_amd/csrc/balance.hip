@@ -35,7 +35,9 @@ constexpr int BL_TILE_BYTES = 72 << 10;  // of a tile: two workgroups share a CU
 constexpr int BL_JOIN = BL_WAVES * (sizeof(float) + sizeof(int));      // bytes a column of a row takes where a workgroup's waves are joined
 constexpr int BL_FINISH = 256;           // threads of the finish
 constexpr int BL_COLUMNS = 4;            // columns of a workgroup of it; the other threads share the partials
-constexpr int BL_BLOCKS = 512;           // most workgroups of a pass: two to a CU, which registers leave room for
+constexpr int BL_BLOCKS = 512;           // workgroups of a pass: two to a CU, which registers leave room for
+constexpr long BL_ROWS = 1024;           // rows that a lane adds in float32, at most about (equal ones are off by half as many roundings); in
+                                         // many long groups, where 512 workgroups would leave more to each, there are more workgroups
 
 struct BalanceArgs {
   const void* x;
@@ -677,15 +679,15 @@ int lanes_per_row(int experts) {
   return lpr;
 }
 
-// workgroups per group: enough rows to fill them, two to a CU over all groups (they walk the rows that are left).  One group whose
-// rows a workgroup has done in four rounds stays with one: that saves the two launches that join partials.
+// workgroups per group: enough rows to fill them, two to a CU over all groups (they walk the rows that are left), more for BL_ROWS.  One
+// group whose rows a workgroup has done in four rounds stays with one: that saves the two launches that join partials.
 long rounds(long rows, int experts) {
   const long per = (long)BL_WAVES * (64 / lanes_per_row(experts));
   return (rows + per - 1) / per;
 }
 int walkers(long groups, long rows, int experts) {
   const long want = rounds(rows, experts), most = groups >= BL_BLOCKS ? 1 : BL_BLOCKS / groups;
-  return (int)(want < 1 ? 1 : want < most ? want : most);
+  return (int)std::max(std::min(std::max(want, 1L), most), (want + BL_ROWS - 1) / BL_ROWS);
 }
 int blocks_for(long groups, long rows, int experts) {
   return groups == 1 && rounds(rows, experts) <= 4 ? 1 : walkers(groups, rows, experts);
