@@ -1948,9 +1948,10 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
                 "adamw_step: moments of parameter ", i, ": both float32, or float8_e4m3fn and float8_e5m2");
     TORCH_CHECK(m.device() == dev && m.sizes() == p.sizes() && same_order(m, p) && v.device() == dev && v.sizes() == p.sizes() && same_order(v, p),
                 "adamw_step: moments of parameter ", i, ": its shape, strides and device");
+    TORCH_CHECK(!p.is_neg() && !m.is_neg() && !v.is_neg(), "adamw_step: parameter ", i, " or a moment of it is a negated view");
     if (p.numel() == 0) continue;
     kinds |= 1 << kind[i];
-    if (same_order(g, p)) {
+    if (same_order(g, p) && !g.is_neg()) {
       const char* from = static_cast<const char*>(g.const_data_ptr());
       reads.emplace_back(from, from + p.nbytes());
     } else {
@@ -1974,6 +1975,7 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
   auto one = [&](const OptTensor& t, at::ScalarType want, const char* what) {
     if (!t.has_value() || !t->defined()) return;
     TORCH_CHECK(t->device() == dev && t->scalar_type() == want && t->numel() == 1, "adamw_step: ", what, ": one ", want, " value on the parameters' device");
+    TORCH_CHECK(!t->is_neg(), "adamw_step: ", what, " is a negated view");
   };
   one(clip, at::kFloat, "clip");
   one(lr_dev, at::kFloat, "a learning rate on the device");
@@ -1981,7 +1983,7 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
   const bool captured = step_dev.has_value() && step_dev->defined(), lr_on_dev = lr_dev.has_value() && lr_dev->defined();
   TORCH_CHECK(captured || !lr_on_dev, "adamw_step: a learning rate on the device needs the step count on the device too");
   const float* clip_p = clip.has_value() && clip->defined() ? clip->data_ptr<float>() : nullptr;
-  // nor is what is written read by other threads (gradients of another order are copied before the first launch)
+  // nor is what is written read by other threads (gradients of another order, and negated views, are copied before the first launch)
   if (clip_p) reads.emplace_back(reinterpret_cast<const char*>(clip_p), reinterpret_cast<const char*>(clip_p + 1));
   TORCH_CHECK(!touches(reads, all), "adamw_step: a gradient or the clip factor shares memory with a parameter or a moment");
   DeviceGuard guard(dev);
@@ -2004,7 +2006,7 @@ void op_adamw_step(const TensorList& params, const TensorList& grads, const Tens
           if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     }
   } bump{{&params, &exp_avgs, &exp_avg_sqs, &exp_avg_scales, &exp_avg_sq_scales}};
-  std::vector<Tensor> hold;                                    // gradients brought into their parameters' order, as they come below
+  std::vector<Tensor> hold;                                    // those gradients, in the order they are taken below
   for (int k = 0; k < 4; ++k)
     for (size_t i = 0; i < n && copies; ++i)
       if (kind[i] == k && copied[i]) {
@@ -2072,7 +2074,7 @@ struct BalanceLoss : public torch::autograd::Function<BalanceLoss> {
     DeviceGuard guard(x.device());
     const bool grouped = x.dim() == 3, masked = mask.defined();
     const int64_t groups = grouped ? x.size(0) : 1, rows = x.size(-2), experts = x.size(-1);
-    Tensor up = grads[0].to(at::kFloat), dx = at::empty_like(x);
+    Tensor up = grads[0].to(at::kFloat).resolve_neg(), dx = at::empty_like(x);
     if (x.numel() == 0) return {dx, Tensor(), Tensor(), Tensor()};
     RM_CALL(repmode_balance_bwd, x.data_ptr(), dtype_code(x.scalar_type()), groups, rows, (int)experts, grouped ? x.stride(0) : 0, x.stride(-2),
             x.stride(-1), masked ? reinterpret_cast<const unsigned char*>(mask.data_ptr<bool>()) : nullptr, masked && grouped ? mask.stride(0) : 0,
@@ -2105,7 +2107,7 @@ std::tuple<Tensor, Tensor, Tensor> op_balance_loss(const Tensor& logits, const O
     TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == at::kBool && mask->sizes() == logits.sizes().slice(0, logits.dim() - 1),
                 "balance_loss: the mask is bool ", logits.sizes().slice(0, logits.dim() - 1), " on the logits' device");
   }
-  auto out = BalanceLoss::apply(logits, mask, top_k, coef);
+  auto out = BalanceLoss::apply(logits.resolve_neg(), mask, top_k, coef);
   return {out[0], out[1], out[2]};
 }
 

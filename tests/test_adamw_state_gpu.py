@@ -150,3 +150,29 @@ def test_what_is_written_moves_its_version():
         if bits == 32:
             with pytest.raises(RuntimeError, match='modified by an inplace operation'):
                 graph.backward()
+
+
+def test_views_that_are_negated_when_read():
+    """Views whose memory holds the negated values (what .imag of a conjugate is): read as what they stand for, not written."""
+    ops = _ops()
+    p, g, s = _fresh(32, (300,), (torch.float32,))
+    neg = torch._neg_view(g[0])
+    assert neg.is_neg() and torch.equal(neg, -g[0])
+    other = [x.clone() for x in (p[0], s[0][0], s[2][0])]
+    ops.adamw_step(p, [neg], s[0], s[2], 1)
+    ops.adamw_step([other[0]], [-g[0]], [other[1]], [other[2]], 1)
+    for a, b in zip((p[0], s[0][0], s[2][0]), other):
+        assert torch.equal(a, b)
+    assert torch.equal(ops.grad_norm([neg])[0], ops.grad_norm(g)[0])
+    x = torch.randn(40, 12, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for a, b in zip(ops.balance_loss(torch._neg_view(x), 3), ops.balance_loss(-x, 3)):
+        assert torch.equal(a, b)
+    up, y = torch.tensor(-2.0, device=DEV), -x
+    grads = [torch.autograd.grad(ops.balance_loss(z, 3)[0], z, grad_outputs=u) for z, u in
+             ((y.requires_grad_(True), -up), (torch._neg_view(x).requires_grad_(True), -up), (y, torch._neg_view(up)))]
+    assert all(torch.equal(a[0], grads[0][0]) for a in grads)
+    for bad in (lambda: ops.adamw_step([torch._neg_view(p[0])], g, s[0], s[2], 1), lambda: ops.adamw_step(p, g, [torch._neg_view(s[0][0])], s[2], 1),
+                lambda: ops.adamw_step(p, g, s[0], [torch._neg_view(s[2][0])], 1),
+                lambda: ops.adamw_step(p, g, s[0], s[2], 1, clip=torch._neg_view(torch.ones((), device=DEV)))):
+        with pytest.raises(RuntimeError, match='negated'):
+            bad()
