@@ -236,12 +236,19 @@ class AdamW(torch.optim.Optimizer):
         """The type a saved moment is kept in: float32 for anything of 16 bits (a stock optimizer's of bfloat16 parameters)."""
         return torch.float32 if v.dtype in (torch.bfloat16, torch.float16) else v.dtype
 
-    def _check_captured(self, state_dict):
-        """Whether a state can go into the tensors that a captured step holds; raises before anything has changed where it cannot."""
+    def _check_loaded(self, state_dict):
+        """Raises, before anything has changed, where 8-bit moments lie in another order than their parameter (their scales are those of
+        neighbours in memory), or where a state does not fit the tensors that a captured step holds."""
         for saved, group in zip(state_dict['param_groups'], self.param_groups):
             counts = set()
             for key, p in zip(saved['params'], group['params']):
                 st, there = state_dict['state'].get(key, {}), self.state.get(p, {})
+                for v in (st.get('exp_avg'), st.get('exp_avg_sq')):
+                    if (torch.is_tensor(v) and v.dtype.itemsize == 1 and v.shape == p.shape and v.stride() != p.stride() and
+                            not (v.is_contiguous() and p.is_contiguous())):
+                        raise ValueError('repmode_amd.optim.AdamW: 8-bit moments whose order in memory is not their parameter\'s')
+                if not self._captured:
+                    continue
                 if st or there:
                     counts.add(int(st.get('step', 0)))
                 if not st or not there:                  # (no moments yet; or none saved: those that are there become zero)
@@ -258,8 +265,7 @@ class AdamW(torch.optim.Optimizer):
         """As torch.optim.AdamW's, with the moments as they were saved.  After a captured step the state goes into the tensors that the
         graph holds -- a parameter without state gets zero moments -- and one that does not fit them is refused.  A group's learning rate
         on the device stays the tensor that it is and takes the loaded value."""
-        if self._captured:
-            self._check_captured(state_dict)
+        self._check_loaded(state_dict)
         self._settle()
         own = [{k: g[k] for k in ('state_bits', 'min_8bit_numel', 'lr')} for g in self.param_groups]
         # (captured steps hold the moments by address, as they do the step counts: what fits goes into the tensors that are there)
@@ -282,7 +288,9 @@ class AdamW(torch.optim.Optimizer):
                     if k == 'step':
                         self.state[p][k] = torch.tensor(float(v))
                     elif torch.is_tensor(v):
-                        v = v.detach().to(p.device, self._kept_as(v), copy=True)
+                        # (a moment of its parameter's shape takes its strides too)
+                        v = torch.empty_like(p if v.shape == p.shape else v, dtype=self._kept_as(v), device=p.device,
+                                             requires_grad=False).copy_(v.detach())
                         there = held.get(p, {}).get(k)
                         if torch.is_tensor(there) and there.dtype == v.dtype and there.shape == v.shape:
                             v = there.copy_(v)

@@ -193,3 +193,36 @@ def test_a_load_forgets_the_step_before_it(monkeypatch):
     opt.load_state_dict(_loaded(32, sizes=(5,), steps=(3,)))
     opt.step()
     assert fake.steps[-1]['step'] == 4 and int(opt.state[p]['step']) == 4
+
+
+@pytest.mark.parametrize('capturable', [False, True])
+def test_moments_saved_in_another_order(monkeypatch, capturable):
+    """float32 moments take their parameter's strides, as torch.optim.AdamW's would; 8-bit ones, whose scales go by the order in memory,
+    are refused where it is another."""
+    from repmode_amd import ops, optim
+    monkeypatch.setattr(ops, 'list_ops', lambda: _FakeOps())
+    shape = (3, 8, 5, 5)
+    def one(fmt, bits, **kw):
+        p = torch.nn.Parameter(torch.zeros(shape).to(memory_format=fmt))
+        p.grad = torch.ones_like(p)
+        opt = optim.AdamW([p], state_bits=bits, min_8bit_numel=1, **kw)
+        opt.step()
+        return opt, p
+    plain, last = torch.contiguous_format, torch.channels_last
+    opt, p = one(plain, 32)
+    opt.state[p]['exp_avg'].copy_(torch.arange(600.).view(shape))
+    into, q = one(last, 32, capturable=capturable)
+    into.load_state_dict(opt.state_dict())
+    for k in ('exp_avg', 'exp_avg_sq'):
+        assert torch.equal(into.state[q][k], opt.state[p][k]) and into.state[q][k].stride() == q.stride()
+    opt, p = one(plain, 8)
+    into, q = one(last, 8, capturable=capturable)
+    was = dict(into.state[q])
+    with pytest.raises(ValueError, match='order'):
+        into.load_state_dict(opt.state_dict())
+    assert all(into.state[q][k] is t for k, t in was.items())
+    other, r = one(last, 8)
+    other.state[r]['exp_avg'].view(torch.uint8).copy_((torch.arange(600) % 120).view(shape))
+    into.load_state_dict(other.state_dict())
+    assert torch.equal(into.state[q]['exp_avg'].view(torch.uint8), other.state[r]['exp_avg'].view(torch.uint8))
+    assert into.state[q]['exp_avg'].stride() == q.stride()

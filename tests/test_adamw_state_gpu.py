@@ -176,3 +176,62 @@ def test_views_that_are_negated_when_read():
                 lambda: ops.adamw_step(p, g, s[0], s[2], 1, clip=torch._neg_view(torch.ones((), device=DEV)))):
         with pytest.raises(RuntimeError, match='negated'):
             bad()
+
+
+def _captured(bits, **kw):
+    """An optimizer over two parameters whose step is in a graph, after one step launch by launch, and a twin without one."""
+    from repmode_amd.optim import AdamW
+    ps, gs, _ = _fresh(bits, dtypes=(torch.float32, torch.float32))
+    a, b = ([torch.nn.Parameter(p.clone()) for p in ps] for _ in range(2))
+    opt = AdamW(a, max_norm=1.0, state_bits=bits, seed=5, capturable=True, **kw)
+    _with_grads(a, gs)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for p, q in zip(a, b):
+        q.data.copy_(p.detach())
+    return graph, opt, a, b, gs
+
+
+@pytest.mark.parametrize('through', ['device', 'host'])
+@pytest.mark.parametrize('bits', [32, 8])
+def test_replays_go_on_from_a_loaded_state(bits, through):
+    """Rewound to a new optimizer's state, then loaded with a twin's, with memory that was freed taken and filled in between: each replay
+    is the twin's step, and a learning rate on the device is the one that a scheduler fills."""
+    from repmode_amd.optim import AdamW
+    graph, opt, a, b, gs = _captured(bits, lr=torch.tensor(1e-2, device=DEV))
+    twin = AdamW(b, lr=float(torch.tensor(1e-2, dtype=torch.float32)), max_norm=1.0, state_bits=bits, seed=5)
+    lr = opt.param_groups[0]['lr']
+    def load(state):
+        opt.load_state_dict({k: v for k, v in state.items()} if through == 'device' else torch.utils._pytree.tree_map(
+            lambda t: t.cpu() if torch.is_tensor(t) else t, state))
+        hold = [torch.full((n,), math.nan, device=DEV) for n in (1, 64, 300, 1280, 5000) for _ in range(20)]
+        torch.cuda.synchronize()
+        del hold
+    def both(n):
+        for t in range(n):
+            for p, g in zip(a, gs):
+                p.grad.copy_(g * (t + 2))
+            _with_grads(b, [g * (t + 2) for g in gs])
+            graph.replay()
+            twin.step()
+            torch.cuda.synchronize()
+            for p, q in zip(a, b):
+                assert torch.equal(p.detach(), q.detach()), t
+                assert all(torch.equal(_bytes(opt.state[p][k]), _bytes(v)) for k, v in twin.state[q].items() if k != 'step')
+    load(twin.state_dict())                              # (no step yet: no moments)
+    both(3)
+    for q, g in zip(b, gs):                              # the twin goes on alone, and then its state is loaded
+        q.grad = g.clone()
+    twin.step()
+    for p, q in zip(a, b):
+        p.data.copy_(q.detach())
+    load(copy.deepcopy(twin.state_dict()))
+    assert opt.param_groups[0]['lr'] is lr
+    both(2)
+    lr.fill_(3e-3)
+    twin.param_groups[0]['lr'] = float(lr)
+    both(2)
+    assert all(int(s['step']) == 8 for s in opt.state_dict()['state'].values())
