@@ -38,6 +38,34 @@ def install_foreign_step_hook():
         _hook_handle = register_optimizer_step_post_hook(_foreign_step_hook)
 
 
+def _capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def _kept_as(v):
+    """The type a saved moment is kept in: float32 for anything of 16 bits (a stock optimizer's of bfloat16 parameters)."""
+    return torch.float32 if v.dtype in (torch.bfloat16, torch.float16) else v.dtype
+
+
+def _check_captured(who, opt, state_dict):
+    """Raises, before anything has changed, where a state does not fit the tensors that a captured step holds."""
+    for saved, group in zip(state_dict['param_groups'], opt.param_groups):
+        counts = set()
+        for key, p in zip(saved['params'], group['params']):
+            st, there = state_dict['state'].get(key, {}), opt.state.get(p, {})
+            if st or there:
+                counts.add(int(st.get('step', 0)))
+            if not st or not there:                      # (no moments yet; or none saved: those that are there become zero)
+                continue
+            new = {k: (_kept_as(v), v.shape) for k, v in st.items() if k != 'step' and torch.is_tensor(v)}
+            if new != {k: (t.dtype, t.shape) for k, t in there.items() if k != 'step'}:
+                raise ValueError('repmode_amd.optim.%s: a captured step holds this optimizer\'s moments, and the state has others (another '
+                                 'number of bits, other shapes): load it into a new optimizer and capture again' % who)
+        if len(counts) > 1:
+            raise ValueError('repmode_amd.optim.%s: a captured step holds one step count for a group, and the state\'s counts differ: load it '
+                             'into a new optimizer and capture again' % who)
+
+
 class Adam(torch.optim.Adam):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, capturable=False):
         """``capturable``: the step count ALSO lives on the device (one int64 for the whole parameter list) and the kernels take
@@ -49,6 +77,7 @@ class Adam(torch.optim.Adam):
                          capturable=False)
         self.device_step = bool(capturable)
         self._step_dev = self._hyper_dev = None
+        self._captured = False       # a step was captured: some graph may hold moments, count and constants by address
 
     def sync_steps(self):
         """Device step count -> the host counters of ``state`` (after graph replays, which run no host code).  One device read."""
@@ -67,16 +96,25 @@ class Adam(torch.optim.Adam):
         copy at load time, so that ``step()`` never reads the device to learn the step count)."""
         if any('exp_avg_scale' in st for st in state_dict['state'].values()):
             raise ValueError('repmode_amd.optim.Adam: these moments are in 8 bits (optim.AdamW)')
+        if self._captured:
+            _check_captured('Adam', self, state_dict)
+        held = {p: dict(st) for p, st in self.state.items()} if self._captured else {}
         super().load_state_dict(state_dict)
+        for p, st in held.items():                 # (what a captured step holds by address takes the loaded values; none: zeros)
+            new = self.state[p]
+            for k in ('exp_avg', 'exp_avg_sq'):
+                st[k].copy_(new[k]) if k in new else st[k].zero_()
+                new[k] = st[k]
+            new.setdefault('step', torch.tensor(0.0))
         for group in self.param_groups:            # (a stock optimizer's groups say fused / capturable; this one's bookkeeping is neither)
             group['fused'], group['capturable'], group['foreach'] = False, False, False
         for st in self.state.values():
             if torch.is_tensor(st.get('step')) and st['step'].is_cuda:
                 st['step'] = st['step'].detach().cpu()
         if self._step_dev is not None:
-            # A captured step holds the device count and the constants' buffer BY ADDRESS (ADVICE round 5): they stay where they
-            # are and take the loaded count in place.  Counters that disagree cannot be one device count: the buffers go, and the
-            # next step says so (as a first step would).
+            # A captured step holds the device count and the constants' buffer BY ADDRESS: they stay where they are and take the
+            # loaded count in place.  Counters that disagree cannot be one device count: where nothing was captured the buffers go,
+            # and the next step says so (as a first step would).
             loaded = {int(st['step']) for st in self.state.values() if 'step' in st}
             if len(loaded) <= 1:
                 self._step_dev.fill_(loaded.pop() if loaded else 0)
@@ -108,10 +146,11 @@ class Adam(torch.optim.Adam):
                     if len(t0) != 1:
                         raise RuntimeError('repmode_amd.optim.Adam(capturable=True): every parameter must have seen the same '
                                            'number of steps')
-                    if torch.cuda.is_current_stream_capturing():
+                    if _capturing():
                         raise RuntimeError('repmode_amd.optim.Adam(capturable=True): run one step launch by launch before capturing')
                     self._step_dev = torch.full((1,), t0.pop(), dtype=torch.int64, device=params[0].device)
                     self._hyper_dev = torch.zeros(8, dtype=torch.float32, device=params[0].device)
+                self._captured |= _capturing()
                 for s in steps:
                     s += 1              # (host mirror: exact while steps run launch by launch; sync_steps() after replays)
                 ops_.torch_ops().adam_step_dev(params, grads, exp_avgs, exp_avg_sqs, lr, float(beta1), float(beta2), float(group['eps']),
@@ -129,10 +168,6 @@ class Adam(torch.optim.Adam):
                 ops_.torch_ops().adam_step(sel(params), sel(grads), sel(exp_avgs), sel(exp_avg_sqs), lr, float(beta1), float(beta2),
                                            float(group['eps']), t)
         return loss
-
-
-def _capturing():
-    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 class AdamW(torch.optim.Optimizer):
@@ -231,35 +266,18 @@ class AdamW(torch.optim.Optimizer):
         self.sync_steps()
         return super().state_dict()
 
-    @staticmethod
-    def _kept_as(v):
-        """The type a saved moment is kept in: float32 for anything of 16 bits (a stock optimizer's of bfloat16 parameters)."""
-        return torch.float32 if v.dtype in (torch.bfloat16, torch.float16) else v.dtype
-
     def _check_loaded(self, state_dict):
         """Raises, before anything has changed, where 8-bit moments lie in another order than their parameter (their scales are those of
         neighbours in memory), or where a state does not fit the tensors that a captured step holds."""
         for saved, group in zip(state_dict['param_groups'], self.param_groups):
-            counts = set()
             for key, p in zip(saved['params'], group['params']):
-                st, there = state_dict['state'].get(key, {}), self.state.get(p, {})
+                st = state_dict['state'].get(key, {})
                 for v in (st.get('exp_avg'), st.get('exp_avg_sq')):
                     if (torch.is_tensor(v) and v.dtype.itemsize == 1 and v.shape == p.shape and v.stride() != p.stride() and
                             not (v.is_contiguous() and p.is_contiguous())):
                         raise ValueError('repmode_amd.optim.AdamW: 8-bit moments whose order in memory is not their parameter\'s')
-                if not self._captured:
-                    continue
-                if st or there:
-                    counts.add(int(st.get('step', 0)))
-                if not st or not there:                  # (no moments yet; or none saved: those that are there become zero)
-                    continue
-                new = {k: (self._kept_as(v), v.shape) for k, v in st.items() if k != 'step' and torch.is_tensor(v)}
-                if new != {k: (t.dtype, t.shape) for k, t in there.items() if k != 'step'}:
-                    raise ValueError('repmode_amd.optim.AdamW: a captured step holds this optimizer\'s moments, and the state has others (another '
-                                     'number of bits, other shapes): load it into a new optimizer and capture again')
-            if len(counts) > 1:
-                raise ValueError('repmode_amd.optim.AdamW: a captured step holds one step count for a group, and the state\'s counts differ: load it '
-                                 'into a new optimizer and capture again')
+        if self._captured:
+            _check_captured('AdamW', self, state_dict)
 
     def load_state_dict(self, state_dict):
         """As torch.optim.AdamW's, with the moments as they were saved.  After a captured step the state goes into the tensors that the
@@ -289,7 +307,7 @@ class AdamW(torch.optim.Optimizer):
                         self.state[p][k] = torch.tensor(float(v))
                     elif torch.is_tensor(v):
                         # (a moment of its parameter's shape takes its strides too)
-                        v = torch.empty_like(p if v.shape == p.shape else v, dtype=self._kept_as(v), device=p.device,
+                        v = torch.empty_like(p if v.shape == p.shape else v, dtype=_kept_as(v), device=p.device,
                                              requires_grad=False).copy_(v.detach())
                         there = held.get(p, {}).get(k)
                         if torch.is_tensor(there) and there.dtype == v.dtype and there.shape == v.shape:

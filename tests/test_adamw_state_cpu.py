@@ -226,3 +226,66 @@ def test_moments_saved_in_another_order(monkeypatch, capturable):
     into.load_state_dict(other.state_dict())
     assert torch.equal(into.state[q]['exp_avg'].view(torch.uint8), other.state[r]['exp_avg'].view(torch.uint8))
     assert into.state[q]['exp_avg'].stride() == q.stride()
+
+
+# ---------------------------------------------------------------------------------------------- the plain Adam
+
+class _FakeAdam:
+    """Stands for the operator library's Adam: the update is left out, but for the moments."""
+
+    def adam_step_dev(self, params, grads, exp_avgs, exp_avg_sqs, *rest):
+        for t in (*exp_avgs, *exp_avg_sqs):
+            t.add_(1)
+
+
+def _captured_adam(monkeypatch):
+    from repmode_amd import ops, optim
+    monkeypatch.setattr(ops, 'torch_ops', lambda: _FakeAdam())
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in (50, 7)]
+    opt = optim.Adam(ps, capturable=True)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    monkeypatch.setattr(torch.cuda, 'is_initialized', lambda: True)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    opt.step()
+    monkeypatch.undo()
+    return opt, ps
+
+
+def _stock_adam(steps=3, sizes=(50, 7)):
+    ps = [torch.nn.Parameter(torch.zeros(n)) for n in sizes]
+    opt = torch.optim.Adam(ps)
+    for t in range(steps):
+        for p in ps:
+            p.grad = torch.full_like(p, t + 1.0)
+        opt.step()
+    return opt, ps
+
+
+def test_a_state_goes_into_what_a_captured_adam_step_holds(monkeypatch):
+    opt, ps = _captured_adam(monkeypatch)
+    held, count, hyper = _tensors(opt, ps), opt._step_dev, opt._hyper_dev
+    stock, qs = _stock_adam()
+    saved = stock.state_dict()
+    opt.load_state_dict(saved)
+    assert all(t is held[k] for k, t in _tensors(opt, ps).items()) and opt._step_dev is count and opt._hyper_dev is hyper and int(count) == 3
+    for p, q in zip(ps, qs):
+        assert all(torch.equal(opt.state[p][k], stock.state[q][k]) for k in ('step', 'exp_avg', 'exp_avg_sq'))
+        assert opt.state[p]['exp_avg'].data_ptr() != stock.state[q]['exp_avg'].data_ptr()
+    opt.load_state_dict(torch.optim.Adam(ps).state_dict())       # (no moments at all: rewound)
+    assert all(t is held[k] and not bool(t.any()) for k, t in _tensors(opt, ps).items()) and int(count) == 0
+    assert opt._step_dev is count and [int(opt.state[p]['step']) for p in ps] == [0, 0]
+
+
+def test_a_state_that_does_not_fit_a_captured_adam_step_is_refused(monkeypatch):
+    opt, ps = _captured_adam(monkeypatch)
+    held, count = _tensors(opt, ps), opt._step_dev
+    opt.load_state_dict(_stock_adam()[0].state_dict())
+    half = _stock_adam(2)[0].state_dict()
+    half['state'][1]['step'] += 1
+    for saved in (half, _stock_adam(sizes=(51, 7))[0].state_dict()):
+        with pytest.raises(ValueError, match='captured'):
+            opt.load_state_dict(saved)
+    assert all(t is held[k] for k, t in _tensors(opt, ps).items()) and opt._step_dev is count and int(count) == 3

@@ -235,3 +235,34 @@ def test_replays_go_on_from_a_loaded_state(bits, through):
     twin.param_groups[0]['lr'] = float(lr)
     both(2)
     assert all(int(s['step']) == 8 for s in opt.state_dict()['state'].values())
+
+
+def test_replays_of_the_plain_adam_go_on_from_a_loaded_state():
+    from repmode_amd.optim import Adam
+    ps, gs, _ = _fresh(32, dtypes=(torch.float32, torch.float32))
+    a, b = ([torch.nn.Parameter(p.clone()) for p in ps] for _ in range(2))
+    opt, twin = Adam(a, lr=1e-2, capturable=True), torch.optim.Adam(b, lr=1e-2)
+    _with_grads(a, gs)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for n in (2, 3):                                     # rewound first, then loaded with the twin's state
+        for p, q in zip(a, b):
+            p.data.copy_(q.detach())
+        opt.load_state_dict(copy.deepcopy(twin.state_dict()))
+        hold = [torch.full((k,), math.nan, device=DEV) for k in (1, 300, 5000) for _ in range(20)]
+        torch.cuda.synchronize()
+        del hold
+        for t in range(n):
+            for p, g in zip(a, gs):
+                p.grad.copy_(g * (t + 2))
+            _with_grads(b, [g * (t + 2) for g in gs])
+            graph.replay()
+            twin.step()
+            torch.cuda.synchronize()
+            for p, q in zip(a, b):
+                # a step moves by lr m / sqrt(v), at most about 1e-2: both sides' roundings of it, and the parameter's
+                assert float((p.detach() - q.detach()).abs().max()) < 5 * (2.0 ** -24 * float(q.detach().abs().max()) + 64 * 2.0 ** -24 * 1e-2)
+    assert int(opt._step_dev) == 5
