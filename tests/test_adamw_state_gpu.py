@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from test_hip_parity import DEV, _ops
-from test_train_ops_gpu import _bytes
+from test_train_ops_gpu import HYPER, _bytes, _check_guards, _grid, _noise, _tensors, _update64
 
 pytestmark = pytest.mark.gpu
 
@@ -266,3 +266,28 @@ def test_replays_of_the_plain_adam_go_on_from_a_loaded_state():
                 # a step moves by lr m / sqrt(v), at most about 1e-2: both sides' roundings of it, and the parameter's
                 assert float((p.detach() - q.detach()).abs().max()) < 5 * (2.0 ** -24 * float(q.detach().abs().max()) + 64 * 2.0 ** -24 * 1e-2)
     assert int(opt._step_dev) == 5
+
+
+@pytest.mark.parametrize('offset', [0, 1])
+@pytest.mark.parametrize('sizes', [(1, 3, 4), (1, 1, 1, 1, 2, 2, 2, 2), (9, 8, 7, 6, 5)])
+def test_bfloat16_parameters_of_a_few_elements(sizes, offset):
+    """Every element of the smallest tensors is the neighbour that its random bits choose (float64 definition), but where those lie
+    within the arithmetic's own error of the border; over all steps nearly none does."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(21)
+    (p, g, m, v), guards = _tensors(sizes, torch.bfloat16, gen, offset)
+    sure_of, total = 0, 0
+    for t in range(1, 30):
+        was = [[x.clone() for x in lst] for lst in (p, g, m, v)]
+        ops.adamw_step(p, g, m, v, t, seed=11, **HYPER)
+        for i, n in enumerate(sizes):
+            p1, _, _, dp, _, _ = _update64(*(lst[i] for lst in was), t, **HYPER)
+            low, step = _grid(p1.abs(), 7, -126)
+            bits = _noise(11, t, i, torch.arange(n))[1].double() / 65536
+            frac = (p1.abs() - low) / step
+            sure = (frac + bits - 1).abs() > dp / step + 2.0 ** -20
+            want = torch.copysign(low + step * (frac + bits >= 1), p1)
+            assert bool((p[i].cpu().double() == want)[sure].all()), (t, i)
+            sure_of, total = sure_of + int(sure.sum()), total + n
+    assert sure_of > 0.9 * total
+    _check_guards([x for x in guards if x[0].dtype == torch.bfloat16])
