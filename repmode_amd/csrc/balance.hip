@@ -105,9 +105,10 @@ template <int LPR, int EPL>
 __device__ __forceinline__ float row_exp(float top, const float (&x)[EPL], float (&y)[EPL]) {
   constexpr float L = 1.44269504f;
   const float shift = top * L;
-  if (__any(fabsf(top) >= 0x1p20f)) {
+  const bool far = fabsf(top) >= 0x1p20f;
+  if (__any(far)) {                                           // (row by row: what a row gives does not go by the rows beside it)
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f((x[j] - top) * L);
+    for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f(far ? (x[j] - top) * L : fmaf(x[j], L, -shift));
   } else {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) y[j] = __builtin_amdgcn_exp2f(fmaf(x[j], L, -shift));

@@ -26,3 +26,24 @@ def test_mean_probabilities_of_long_groups(experts, rows, dtype):
     assert torch.equal(counts.cpu(), want.expand(257, experts))
     assert float(((prob.double().cpu() - p) / p).abs().max()) <= most
     assert abs(float(loss) - experts * float(p.max())) <= most * experts * float(p.max())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('experts', [5, 24, 200, 600])
+def test_a_row_does_not_go_by_the_rows_beside_it(experts, dtype):
+    """The gradient of ordinary rows is the same, bit by bit, whether other rows lie near zero or far from it (where the softmax takes
+    its difference to the maximum in two steps), as long as those choose alike."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(64, experts, generator=gen).to(dtype)
+    moved = x.clone()
+    moved[::3] = torch.where(torch.arange(experts) == x[::3].float().argmax(1, keepdim=True), 1e9, -1e9).to(dtype)
+    keep = torch.ones(64, dtype=torch.bool)
+    keep[::3] = False
+    out = []
+    for z in (x, moved):
+        z = z.to(DEV).requires_grad_(True)
+        loss, counts, _ = ops.balance_loss(z, 1)
+        grad, = torch.autograd.grad(loss, z)
+        out.append((counts, grad.cpu()[keep]))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1]) and bool(torch.isfinite(out[0][1]).all())
