@@ -19,7 +19,7 @@
 //
 // What bounds both: HBM.  float32 moments move 28 B an element (bfloat16 parameters: 22), 8-bit ones 16 (10).  108.6 M float32 parameters
 // 517 us (5.9 TB/s; four reads and three writes without arithmetic reach that too) and, 8-bit moments, 283 us (6.1); 201 M bfloat16
-// ones 750 us (5.9), 402.8 M with 8-bit moments 670 us (6.0).  With bfloat16 parameters and 8-bit moments the vector units are next:
+// ones 750 us (5.9), 402.8 M with 8-bit moments 682 us (5.9).  With bfloat16 parameters and 8-bit moments the vector units are next:
 // hence one first hash multiplication for four elements, and the hardware's stochastic conversions.
 #include "common.h"
 
