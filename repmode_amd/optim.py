@@ -234,7 +234,7 @@ class AdamW(torch.optim.Optimizer):
         event = None
         if clip.is_cuda:
             if self._flag is None:
-                self._flag = torch.empty((), dtype=torch.float32, pin_memory=True), torch.cuda.Event()
+                self._flag = torch.empty((), dtype=torch.float32, device='cpu', pin_memory=True), torch.cuda.Event()
             (flag, event), stream = self._flag, torch.cuda.current_stream(clip.device)
             clip = flag.copy_(clip, non_blocking=True)
             event.record(stream)

@@ -291,3 +291,16 @@ def test_bfloat16_parameters_of_a_few_elements(sizes, offset):
             sure_of, total = sure_of + int(sure.sum()), total + n
     assert sure_of > 0.9 * total
     _check_guards([x for x in guards if x[0].dtype == torch.bfloat16])
+
+
+def test_the_look_at_the_last_step_under_another_default_device():
+    """What is copied to the host lies there whatever device new tensors go to by default."""
+    from repmode_amd.optim import AdamW
+    _ops()
+    p = torch.nn.Parameter(torch.ones(8, device=DEV))
+    opt = AdamW([p], max_norm=1.0)
+    with torch.device(DEV):
+        for g, want in ((math.inf, 0), (1.0, 1), (math.nan, 1), (1.0, 2)):
+            p.grad = torch.full((8,), g)
+            opt.step()
+            assert int(opt.state_dict()['state'][0]['step']) == want
